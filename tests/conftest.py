@@ -26,3 +26,14 @@ def _restore_torch_threads():
     yield
     if torch.get_num_threads() != n:
         torch.set_num_threads(n)
+
+
+@pytest.fixture(autouse=True)
+def _restore_arithmetic():
+    """The kernels' arithmetic is process state (ops.set_geo_mode and its like): a test leaves it as it found it, whatever its own fixtures set."""
+    from spurfies_amd import ops
+
+    arith, h2 = dict(ops._ARITH), dict(ops._H2)
+    yield
+    ops._ARITH.update(arith)
+    ops._H2.update(h2)
