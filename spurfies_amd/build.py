@@ -19,8 +19,10 @@ SOURCES = ["grid.hip", "geo_mlp.hip", "color_mlp.hip", "rhead_mlp.hip", "wgrad.h
 # 128 registers per wave tile) into AGPRs and paid a v_accvgpr_read per element in every epilogue — 21 % of the geometry kernel's vector
 # instructions, 12 - 14 % of the colour / head kernels' (static counts: geo main pass 12 445 -> 10 417 VALU, head backward 6 222 -> 5 467); the
 # kernels are VALU- and power-bound beside the matrix pipe, so the step went 3.45 -> 3.29 ms on one box (A B B A B A).  No scratch in any kernel.
+# -packed-fp32-ops: no packed fp32 arithmetic (v_pk_add / mul / fma_f32), which -O3 makes from ordinary float code; some of its forms have given wrong
+# results now and then, with no error.  Every product and sum rounds as before (host passes warn that they do not know the feature: harmless).
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
-         "-mllvm", "-amdgpu-mfma-vgpr-form", "-Wall", "-Wno-unused-function"]
+         "-mllvm", "-amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]
 FLAGS_STAMP = os.path.join(LIBDIR, "build_flags.txt")      # objects built with other flags are stale
 
 

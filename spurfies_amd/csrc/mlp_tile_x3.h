@@ -340,22 +340,14 @@ __device__ __forceinline__ f32x16 gemm_x3_tile(const __bf16* X, int n, gx3 wp, i
     return hi;
 }
 
-// ---- epilogue arithmetic, two elements per instruction where the ISA allows (v_cvt_pk_bf16_f32, v_pk_add_f32, v_pk_mul_f32) ----
+// ---- epilogue arithmetic, two elements per instruction where that is safe (v_cvt_pk_bf16_f32; fp32 sums and products stay scalar: the library is built
+// without the packed fp32 instructions, some of whose forms have given wrong results now and then) ----
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// (the compiler pairs the subtractions of the split on its own, but scalarises sums / products whose results feed inline asm)
-__device__ __forceinline__ f32x2 pk_add(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 pk_mul(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("v_pk_mul_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
+__device__ __forceinline__ f32x2 pk_add(f32x2 a, f32x2 b) { return f32x2{a[0] + b[0], a[1] + b[1]}; }
+__device__ __forceinline__ f32x2 pk_mul(f32x2 a, f32x2 b) { return f32x2{a[0] * b[0], a[1] * b[1]}; }
 // h = a + b and 0.01 h for four accumulator values
 __device__ __forceinline__ void bias_scale4(const f32x16& acc, int g, f32x4 b, f32x4& h, f32x4& hs) {
     const f32x2 c = f32x2{0.01f, 0.01f};
