@@ -16,7 +16,7 @@
  *   - Return value: 0 on success, negative SPF_E* code otherwise; text in spf_last_error()
  *     (thread-local).  No exceptions cross the ABI.
  *   - All floating-point data is float32 (the reference forces fp32, spurfies/train.py:23-24),
- *     indices are int32.
+ *     indices are int32; only the operators that take a `type` argument also take bf16 and fp16.
  */
 #ifndef SPURFIES_HIP_H
 #define SPURFIES_HIP_H
@@ -741,6 +741,58 @@ int64_t spf_adam_workspace_floats(void);
  * workspace: spf_adam_workspace_floats() floats.  Two launches, no host synchronisation. */
 int spf_adam_step(float* param, float* grad, float* exp_avg, float* exp_avg_sq, int64_t n, double lr, double beta1,
                   double beta2, double eps, double max_norm, int32_t zero_grads, float* state, float* workspace, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Training operators of normalised MLP layers whose saved activations are held in 8 bits.  No counterpart in the reference, whose networks
+ * (spurfies/model/pointneus_disent.py:73-107) keep every activation in fp32: these are for wider or deeper heads beside them.
+ * Matrices are rows of `cols` consecutive elements, `ld*` elements apart (an input's row stride may be 0: a broadcast row), of one of
+ * the three element types; any column count and any element-aligned address.  rows == 0 or cols == 0: nothing is launched or written.
+ * ---------------------------------------------------------------------------------------- */
+#define SPF_TYPE_F32 0
+#define SPF_TYPE_BF16 1
+#define SPF_TYPE_F16 2
+
+/* The 8-bit form of a matrix: `codes` [rows][32 * blocks], 16-byte aligned, and `steps` [rows][blocks], blocks = ceil(cols / 32).  The 32 columns of
+ * a block share the step 2^s, s the least for which the block's largest magnitude rounds to at most 127 steps, kept in -126 .. 121 and
+ * stored as the byte s + 127.  A code's low seven bits are the element's magnitude in steps, to nearest with ties to even (off by at most
+ * half a step; at most one where s = 121); its top bit is set where the element is not greater than zero.  A block that holds an infinity
+ * or a NaN has the step byte 255 and stands for NaN.  Codes behind a row's last column are 0. */
+int spf_saved8_pack(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* steps, void* stream);
+/* Values beyond fp16's range come back as +-65504 when type is SPF_TYPE_F16. */
+int spf_saved8_restore(const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t cols, void* out, int32_t type, int64_t ldo, void* stream);
+
+/* y = f(x), computed in fp32 and rounded once.  param: LeakyReLU's slope >= 0, softplus' beta > 0 (log(1 + e^(beta x)) / beta), else unused.
+ * in_codes / in_steps (both or neither): the 8-bit form of x.  out_codes / out_steps (both or neither): that of y as stored.
+ * The backward pass reads x's for softplus, SiLU and GELU (the erf form), y's for LeakyReLU (the sign of a code is the sign of x: that
+ * derivative is exact; at x = 0 it is the slope). */
+#define SPF_ACT_LEAKY_RELU 0
+#define SPF_ACT_SOFTPLUS 1
+#define SPF_ACT_SILU 2
+#define SPF_ACT_GELU 3
+int spf_act8_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, int32_t kind, float param, void* y, int64_t ldy,
+                     uint8_t* in_codes, uint8_t* in_steps, uint8_t* out_codes, uint8_t* out_steps, void* stream);
+/* dx = dy * f'(restored) */
+int spf_act8_backward(const void* dy, int32_t type, int64_t ldy, int64_t rows, int64_t cols, int32_t kind, float param, const uint8_t* codes,
+                      const uint8_t* steps, void* dx, int64_t ldx, void* stream);
+
+/* y = (x - mean) rstd weight + bias over each row, rstd = 1 / sqrt(variance + eps) (variance over cols); weight / bias [cols] of type wtype or NULL
+ * (1 and 0); wtype is type or SPF_TYPE_F32.  mean, rstd [rows] (both or neither): what the backward pass reads.  in_* / out_*: the 8-bit forms of x and of y, as above. */
+int spf_layer_norm_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, const void* weight, const void* bias,
+                           int32_t wtype, float eps, void* y, int64_t ldy, float* mean, float* rstd, uint8_t* in_codes, uint8_t* in_steps,
+                           uint8_t* out_codes, uint8_t* out_steps, void* stream);
+int64_t spf_layer_norm_workspace_floats(int64_t rows, int64_t cols);
+/* From dy and one of x and its 8-bit form (the other NULL): dx, dweight, dbias, each or NULL.  dweight / dbias [cols] of type wtype;
+ * accumulate != 0 adds to them.  workspace: spf_layer_norm_workspace_floats() floats, needed for dweight / dbias.  Bit-reproducible. */
+int spf_layer_norm_backward(const void* dy, int32_t type, int64_t ldd, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                            const uint8_t* codes, const uint8_t* steps, const float* mean, const float* rstd, const void* weight, int32_t wtype,
+                            void* dx, int64_t lddx, void* dweight, void* dbias, int32_t accumulate, float* workspace, void* stream);
+
+/* dw [n][cols] = g^T a and db [n] (or NULL) = column sums of g, for g [rows][n] and a [rows][cols] in its 8-bit form: the weight and bias
+ * gradient of a linear layer.  Products are exact, sums fp32, one rounding to wtype; accumulate != 0 adds to dw / db.  A row of g or a
+ * block of a that is not finite gives NaN.  workspace: spf_wgrad8_workspace_floats() floats.  Bit-reproducible. */
+int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols);
+int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols,
+               void* dw, void* db, int32_t wtype, int32_t accumulate, float* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,7 @@ class GridInfo(C.Structure):
 
 _P = C.c_void_p
 _I = C.c_int32
+_L = C.c_int64
 _F = C.c_float
 
 # name -> (restype, argtypes): exactly the entry points of include/spurfies_hip.h
@@ -128,6 +129,15 @@ SIGNATURES = {
     "spf_loss_backward_finalize": (C.c_int, [_P, C.POINTER(LossWeights), _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P,
                                              _P, _P, _P, _P, _I, _P, C.POINTER(LocalTermsArgs), _P]),
     "spf_loss_backward": (C.c_int, [_P, _P, C.POINTER(LossWeights), _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, C.POINTER(LocalTermsArgs), _P]),
+    "spf_saved8_pack": (C.c_int, [_P, _I, _L, _L, _L, _P, _P, _P]),
+    "spf_saved8_restore": (C.c_int, [_P, _P, _L, _L, _P, _I, _L, _P]),
+    "spf_act8_forward": (C.c_int, [_P, _I, _L, _L, _L, _I, _F, _P, _L, _P, _P, _P, _P, _P]),
+    "spf_act8_backward": (C.c_int, [_P, _I, _L, _L, _L, _I, _F, _P, _P, _P, _L, _P]),
+    "spf_layer_norm_forward": (C.c_int, [_P, _I, _L, _L, _L, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _P, _P, _P]),
+    "spf_layer_norm_workspace_floats": (C.c_int64, [_L, _L]),
+    "spf_layer_norm_backward": (C.c_int, [_P, _I, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _P, _L, _P, _P, _I, _P, _P]),
+    "spf_wgrad8_workspace_floats": (C.c_int64, [_L, _L, _L]),
+    "spf_wgrad8": (C.c_int, [_P, _I, _L, _P, _P, _L, _L, _L, _P, _P, _I, _I, _P, _P]),
 }
 
 _lib = None

@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libspurfies_hip.so")
-SOURCES = ["grid.hip", "geo_mlp.hip", "color_mlp.hip", "rhead_mlp.hip", "wgrad.hip", "render.hip", "sampler.hip", "latents.hip", "camera.hip", "loss.hip", "local.hip", "optim.hip"]
+SOURCES = ["grid.hip", "geo_mlp.hip", "color_mlp.hip", "rhead_mlp.hip", "wgrad.hip", "render.hip", "sampler.hip", "latents.hip", "camera.hip", "loss.hip", "local.hip", "optim.hip", "act8.hip", "norm.hip", "wgrad8.hip"]
 # -amdgpu-mfma-vgpr-form (round 6): MFMA accumulators in architectural VGPRs.  The compiler's default put the H2 kernels' accumulators (main + cross:
 # 128 registers per wave tile) into AGPRs and paid a v_accvgpr_read per element in every epilogue — 21 % of the geometry kernel's vector
 # instructions, 12 - 14 % of the colour / head kernels' (static counts: geo main pass 12 445 -> 10 417 VALU, head backward 6 222 -> 5 467); the

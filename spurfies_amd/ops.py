@@ -1567,3 +1567,342 @@ class FusedLoss(_GradModeFunction):
         g_tv_out = None if g_tv is None else (g_tv.expand(n_tv) if n_tv else g_tv.reshape(()))      # per-point array: one value, stride 0
         return (g_rgb, g_acc.view(acc_shape), None if g_psdf is None else g_psdf.view(psdf_shape), g_tv_out,
                 None, None, None, None, None, None, None, None, None, None, None, None, None)
+
+
+# ---- training operators with 8-bit saved activations ------------------------------------------------------------------------------------------
+# Layer norm, activations and the weight gradient of a linear layer for normalised MLP stacks beside the fused networks above: what the backward
+# pass needs of a layer's input is kept in one byte an element (plus one per 32) instead of four or two.  fp32, bf16 and fp16; gradients
+# of parameters go into their sinks (set_grad_sinks) where those are set.  Nothing is cached between calls: workspaces come from the allocator, so
+# captured steps and streams never share one.
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}             # SPF_TYPE_*
+_ACTS = {"leaky_relu": (0, 0.01), "softplus": (1, 1.0), "silu": (2, None), "gelu": (3, None)}      # SPF_ACT_*, the parameter's default
+
+
+def _type_of(t, who):
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise ValueError(f"{who}: needs a tensor on the GPU (the kernels have no CPU form)")
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{who}: float32, bfloat16 or float16 is supported, got {t.dtype}")
+    return _TYPES[t.dtype]
+
+
+def _rows_of(t, who):
+    """t as rows of consecutive elements: (2-D tensor, row stride); a view wherever the strides allow it."""
+    if t.dim() == 0:
+        raise ValueError(f"{who}: needs at least one dimension")
+    cols = t.shape[-1]
+    if t.numel() == 0:
+        rows = 1
+        for n in t.shape[:-1]:
+            rows *= n
+        return t.new_empty((rows, cols)), cols
+    if cols > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    m = t if t.dim() == 2 else t.reshape(-1, cols)
+    if cols > 1 and m.stride(-1) != 1:
+        m = m.contiguous()
+    return m, (m.stride(0) if m.shape[0] > 1 else cols)
+
+
+def _once(who):
+    """In a backward pass: refuse create_graph=True (a gradient of these gradients would lack the saved activations' part)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: the backward pass is not differentiable (create_graph=True)")
+
+
+def _same_device(who, *tensors):
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) > 1:
+        raise ValueError(f"{who}: tensors on different devices: {sorted(map(str, devs))}")
+
+
+class Checkpoint8:
+    """A matrix of activations in 8 bits (include/spurfies_hip.h: spf_saved8_pack): codes [rows, 32 * blocks] and steps [rows, blocks], uint8.
+    Blocks of 32 columns share a power-of-two step; an element is a sign and a magnitude of seven bits, off by at most half a step (a 127th of
+    the block's largest magnitude, a 64th at worst, is a step).  A block with an infinity or a NaN is restored as NaN."""
+
+    __slots__ = ("codes", "steps", "cols", "dtype", "shape")
+
+    def __init__(self, codes, steps, cols, dtype=torch.float32, shape=None):
+        blocks = -(-cols // 32)
+        if dtype not in _TYPES:
+            raise ValueError(f"Checkpoint8: float32, bfloat16 or float16 is supported, got {dtype}")
+        if (codes.dtype != torch.uint8 or steps.dtype != torch.uint8 or codes.dim() != 2 or steps.dim() != 2 or codes.shape[1] != 32 * blocks or
+                steps.shape != (codes.shape[0], blocks)):
+            raise ValueError(f"Checkpoint8: {cols} columns need uint8 codes [rows, {32 * blocks}] and steps [rows, {blocks}], got {tuple(codes.shape)} and "
+                             f"{tuple(steps.shape)}")
+        if not codes.is_contiguous() or not steps.is_contiguous():
+            raise ValueError("Checkpoint8: codes and steps must be contiguous")
+        _same_device("Checkpoint8", codes, steps)
+        if codes.data_ptr() % 16:
+            raise ValueError("Checkpoint8: codes must be 16-byte aligned")
+        shape = tuple(shape) if shape is not None else (codes.shape[0], cols)
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        if not shape or shape[-1] != cols or rows != codes.shape[0]:
+            raise ValueError(f"Checkpoint8: {codes.shape[0]} rows of {cols} columns are not of the shape {shape}")
+        self.codes, self.steps, self.cols, self.dtype, self.shape = codes, steps, cols, dtype, shape
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.steps.numel()
+
+    def restore(self, dtype=None):
+        """The values it stands for (spf_saved8_restore); dtype: that of the tensor that was saved, unless given."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise ValueError(f"Checkpoint8.restore: float32, bfloat16 or float16 is supported, got {dtype}")
+        if not self.codes.is_cuda:
+            raise ValueError("Checkpoint8.restore: needs tensors on the GPU (the kernels have no CPU form)")
+        dev = self.codes.device
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().spf_saved8_restore(_lib.ptr(self.codes), _lib.ptr(self.steps), self.rows, self.cols, _lib.ptr(out), _TYPES[dtype], self.cols,
+                                                     _lib.stream_ptr()), "spf_saved8_restore")
+        return out
+
+
+def _empty8(rows, cols, dev):
+    blocks = -(-cols // 32)
+    return torch.empty((rows, 32 * blocks), dtype=torch.uint8, device=dev), torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
+
+
+def checkpoint8(x) -> Checkpoint8:
+    """x [..., cols] in 8 bits (spf_saved8_pack).  No gradient flows through it."""
+    code = _type_of(x, "checkpoint8")
+    m, ld = _rows_of(x.detach(), "checkpoint8")
+    codes, steps = _empty8(m.shape[0], m.shape[1], x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().spf_saved8_pack(_lib.ptr(m), code, ld, m.shape[0], m.shape[1], _lib.ptr(codes), _lib.ptr(steps), _lib.stream_ptr()), "spf_saved8_pack")
+    return Checkpoint8(codes, steps, m.shape[1], x.dtype, x.shape)
+
+
+class _Act8(_GradModeFunction):
+    @staticmethod
+    def forward(ctx, x, kind, param, out8):
+        code = _TYPES[x.dtype]
+        m, ld = _rows_of(x, "act8")
+        rows, cols = m.shape
+        dev = x.device
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        train = _GradModeFunction._outer_grad_mode and ctx.needs_input_grad[0]
+        by_output = kind == _ACTS["leaky_relu"][0]            # the sign of y is the sign of x: one 8-bit form serves both this layer and the next
+        in8 = _empty8(rows, cols, dev) if train and not by_output else (None, None)
+        o8 = _empty8(rows, cols, dev) if out8 or (train and by_output) else (None, None)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().spf_act8_forward(_lib.ptr(m), code, ld, rows, cols, kind, param, _lib.ptr(y), cols, *[_lib.ptr(t) for t in in8 + o8],
+                                                   _lib.stream_ptr()), "spf_act8_forward")
+        if train:
+            ctx.save_for_backward(*(o8 if by_output else in8))
+            ctx.kind, ctx.param = kind, param
+        if not out8:
+            return y
+        ctx.mark_non_differentiable(*o8)
+        return (y,) + o8
+
+    @staticmethod
+    def backward(ctx, g, *_):
+        _once("act8")
+        codes, steps = ctx.saved_tensors
+        dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        m, ld = _rows_of(g, "act8")
+        with torch.cuda.device(g.device):
+            _lib.check(_lib.lib().spf_act8_backward(_lib.ptr(m), _TYPES[g.dtype], ld, m.shape[0], m.shape[1], ctx.kind, ctx.param, _lib.ptr(codes), _lib.ptr(steps),
+                                                    _lib.ptr(dx), m.shape[1], _lib.stream_ptr()), "spf_act8_backward")
+        return dx, None, None, None
+
+
+def act8(x, kind, param=None, out8=False):
+    """y = f(x), f one of 'leaky_relu' (param: slope >= 0, default 0.01), 'softplus' (param: beta > 0, default 1), 'silu', 'gelu' (the erf form),
+    whose backward pass reads x in 8 bits (for leaky_relu: y, whose sign is x's, so that its derivative is exact).  out8: -> (y, Checkpoint8 of y),
+    written in the same pass, for the linear8 that follows."""
+    _type_of(x, "act8")
+    if kind not in _ACTS:
+        raise ValueError(f"act8: {kind!r} is none of {sorted(_ACTS)}")
+    number, default = _ACTS[kind]
+    if param is not None and default is None:
+        raise ValueError(f"act8: {kind} has no parameter")
+    param = float(default or 0.0) if param is None else float(param)
+    if kind == "leaky_relu" and not 0.0 <= param < float("inf"):
+        raise ValueError("act8: leaky_relu needs a slope >= 0")
+    if kind == "softplus" and not 0.0 < param < float("inf"):
+        raise ValueError("act8: softplus needs beta > 0")
+    if x.dim() == 0:
+        raise ValueError("act8: needs at least one dimension")
+    if not out8:
+        return _Act8.apply(x, number, param, False)
+    y, codes, steps = _Act8.apply(x, number, param, True)
+    return y, Checkpoint8(codes, steps, x.shape[-1], x.dtype, x.shape)
+
+
+class _LayerNorm(_GradModeFunction):
+    @staticmethod
+    def forward(ctx, x, w, b, eps, saved8, out8):
+        code = _TYPES[x.dtype]
+        m, ld = _rows_of(x, "layer_norm")
+        rows, cols = m.shape
+        dev = x.device
+        wtype = _TYPES[(w if w is not None else b if b is not None else x).dtype]
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        train = _GradModeFunction._outer_grad_mode and any(ctx.needs_input_grad[:3])
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=dev) if train else (None, None)
+        in8 = _empty8(rows, cols, dev) if train and saved8 else (None, None)
+        o8 = _empty8(rows, cols, dev) if out8 else (None, None)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().spf_layer_norm_forward(_lib.ptr(m), code, ld, rows, cols, _lib.ptr(w), _lib.ptr(b), wtype, eps, _lib.ptr(y), cols, _lib.ptr(mean),
+                                                         _lib.ptr(rstd), *[_lib.ptr(t) for t in in8 + o8], _lib.stream_ptr()), "spf_layer_norm_forward")
+        if train:
+            keep_x = None if saved8 else (x if m.data_ptr() == x.data_ptr() else m)
+            ctx.save_for_backward(keep_x, mean, rstd, w, *in8)
+            ctx.wtype, ctx.bias = wtype, b is not None
+            sinks = [_sink(t) if t is not None and need else None for t, need in zip((w, b), ctx.needs_input_grad[1:3])]
+            needed = [s for s, need in zip(sinks, ctx.needs_input_grad[1:3]) if need]
+            ctx.sinks = sinks if needed and all(s is not None for s in needed) else None
+        if not out8:
+            return y
+        ctx.mark_non_differentiable(*o8)
+        return (y,) + o8
+
+    @staticmethod
+    def backward(ctx, g, *_):
+        _once("layer_norm")
+        x, mean, rstd, w, codes, steps = ctx.saved_tensors
+        dev = g.device
+        m, ld = _rows_of(g, "layer_norm")
+        rows, cols = m.shape
+        mx, ldx = (None, 0) if x is None else _rows_of(x, "layer_norm")
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(g.shape, dtype=g.dtype, device=dev) if need_x else None
+        wdtype = {v: k for k, v in _TYPES.items()}[ctx.wtype]
+        new = torch.zeros if rows == 0 else torch.empty
+        dw, db = ctx.sinks if ctx.sinks is not None else [new((cols,), dtype=wdtype, device=dev) if need else None for need in (need_w, need_b)]
+        with torch.cuda.device(dev):
+            l = _lib.lib()
+            ws = torch.empty((int(l.spf_layer_norm_workspace_floats(rows, cols)),), dtype=torch.float32, device=dev) if need_w or need_b else None
+            _lib.check(l.spf_layer_norm_backward(_lib.ptr(m), _TYPES[g.dtype], ld, rows, cols, _lib.ptr(mx), ldx, _lib.ptr(codes), _lib.ptr(steps), _lib.ptr(mean),
+                                                 _lib.ptr(rstd), _lib.ptr(w), ctx.wtype, _lib.ptr(dx), cols, _lib.ptr(dw), _lib.ptr(db),
+                                                 int(ctx.sinks is not None), _lib.ptr(ws), _lib.stream_ptr()), "spf_layer_norm_backward")
+        return (dx,) + ((None, None) if ctx.sinks is not None else (dw, db)) + (None, None, None)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
+    """Layer norm over x's last dimension; weight / bias [cols] (each or None) of x's type or fp32.  saved8: the backward pass reads x in 8 bits
+    (mean and variance are the exact x's) and x itself is not kept.  out8: -> (y, Checkpoint8 of y), written in the same pass."""
+    _type_of(x, "layer_norm")
+    if x.dim() == 0:
+        raise ValueError("layer_norm: needs at least one dimension")
+    params = [t for t in (weight, bias) if t is not None]
+    for t in params:
+        _type_of(t, "layer_norm")
+        if t.shape != x.shape[-1:] or not t.is_contiguous():
+            raise ValueError(f"layer_norm: weight and bias must be contiguous and of the shape {tuple(x.shape[-1:])}, got {tuple(t.shape)}")
+        if t.dtype != params[0].dtype or t.dtype not in (x.dtype, torch.float32):
+            raise ValueError("layer_norm: weight and bias share one type, x's or float32")
+    _same_device("layer_norm", x, *params)
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("layer_norm: eps must be finite and not negative")
+    if not out8:
+        return _LayerNorm.apply(x, weight, bias, eps, bool(saved8), False)
+    y, codes, steps = _LayerNorm.apply(x, weight, bias, eps, bool(saved8), True)
+    return y, Checkpoint8(codes, steps, x.shape[-1], x.dtype, x.shape)
+
+
+def _wgrad8_into(m, ld, codes, steps, cols, dw, db, accumulate):
+    rows, n = m.shape
+    dev = m.device
+    with torch.cuda.device(dev):
+        l = _lib.lib()
+        ws = torch.empty((int(l.spf_wgrad8_workspace_floats(rows, n, cols)),), dtype=torch.float32, device=dev)
+        _lib.check(l.spf_wgrad8(_lib.ptr(m), _TYPES[m.dtype], ld, _lib.ptr(codes), _lib.ptr(steps), rows, n, cols, _lib.ptr(dw), _lib.ptr(db), _TYPES[dw.dtype],
+                                int(accumulate), _lib.ptr(ws), _lib.stream_ptr()), "spf_wgrad8")
+
+
+def wgrad8(g, saved, out=None, dbias=None, bias=True):
+    """(dW [n, cols], db [n]) of a linear layer from the gradient g [..., n] of its output and its saved input (spf_wgrad8): dW = g^T a, db = column sums.
+    New fp32 tensors — bias=False: db is None — or, with out (and dbias), += into those (one type, any of the three; contiguous)."""
+    _type_of(g, "wgrad8")
+    if not isinstance(saved, Checkpoint8):
+        raise ValueError("wgrad8: saved must be a Checkpoint8")
+    m, ld = _rows_of(g.detach(), "wgrad8")
+    rows, n = m.shape
+    if rows != saved.rows:
+        raise ValueError(f"wgrad8: {rows} rows of g against {saved.rows} saved ones")
+    if saved.cols == 0:
+        raise ValueError("wgrad8: the saved input has no columns")
+    if out is None and dbias is not None:
+        raise ValueError("wgrad8: dbias without out")
+    for t, shape in ((out, (n, saved.cols)), (dbias, (n,))):
+        if t is not None:
+            _type_of(t, "wgrad8")
+            if tuple(t.shape) != shape or not t.is_contiguous() or t.dtype != out.dtype:
+                raise ValueError(f"wgrad8: out / dbias must be contiguous, of one type and of the shapes {(n, saved.cols)} / {(n,)}")
+    _same_device("wgrad8", g, saved.codes, out, dbias)
+    if out is not None:
+        _wgrad8_into(m, ld, saved.codes, saved.steps, saved.cols, out, dbias, True)
+        return out, dbias
+    new = torch.zeros if rows == 0 else torch.empty
+    dw = new((n, saved.cols), dtype=torch.float32, device=g.device)
+    db = new((n,), dtype=torch.float32, device=g.device) if bias else None
+    _wgrad8_into(m, ld, saved.codes, saved.steps, saved.cols, dw, db, False)
+    return dw, db
+
+
+class _Linear8(_GradModeFunction):
+    @staticmethod
+    def forward(ctx, x, w, b, codes, steps):
+        y = torch.nn.functional.linear(x, w, b)               # a plain product: the library's
+        if _GradModeFunction._outer_grad_mode and any(ctx.needs_input_grad[:3]):
+            if codes is None and any(ctx.needs_input_grad[1:3]):
+                ck = checkpoint8(x)
+                codes, steps = ck.codes, ck.steps
+            ctx.save_for_backward(w, codes, steps)
+            sinks = [_sink(t) if t is not None and need else None for t, need in zip((w, b), ctx.needs_input_grad[1:3])]
+            needed = [s for s, need in zip(sinks, ctx.needs_input_grad[1:3]) if need]
+            ctx.sinks = sinks if ctx.needs_input_grad[1] and all(s is not None for s in needed) else None
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        _once("linear8")
+        w, codes, steps = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        m, ld = _rows_of(g, "linear8")
+        n, cols = w.shape
+        dx = (m @ w).view(g.shape[:-1] + (cols,)) if need_x else None
+        if not need_w and not need_b:
+            return dx, None, None, None, None
+        if ctx.sinks is not None:
+            _wgrad8_into(m, ld, codes, steps, cols, ctx.sinks[0], ctx.sinks[1], True)
+            return dx, None, None, None, None
+        new = torch.zeros if m.shape[0] == 0 else torch.empty
+        dw = new((n, cols), dtype=w.dtype, device=g.device)
+        db = new((n,), dtype=w.dtype, device=g.device) if need_b else None
+        _wgrad8_into(m, ld, codes, steps, cols, dw, db, False)
+        return dx, (dw if need_w else None), db, None, None
+
+
+def linear8(x, weight, bias=None, saved=None):
+    """y = x weight^T + bias, whose backward pass forms the weight and bias gradients from x in 8 bits; x itself is not kept.  saved: the Checkpoint8 of
+    x that layer_norm(out8=True) or act8(out8=True) wrote beside it (else x is packed here).  x, weight [n, cols] and bias [n] share one type."""
+    _type_of(x, "linear8")
+    if x.dim() == 0 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or (bias is not None and bias.shape != weight.shape[:1]):
+        raise ValueError("linear8: needs x [..., cols], weight [n, cols] and bias [n]")
+    if x.shape[-1] == 0:
+        raise ValueError("linear8: x has no columns")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise ValueError("linear8: x, weight and bias share one type")
+    _same_device("linear8", x, weight, bias, None if saved is None else saved.codes)
+    if saved is not None:
+        rows = 1
+        for k in x.shape[:-1]:
+            rows *= k
+        if not isinstance(saved, Checkpoint8) or saved.rows != rows or saved.cols != x.shape[-1]:
+            raise ValueError("linear8: saved must be the Checkpoint8 of x")
+    return _Linear8.apply(x, weight, bias, None if saved is None else saved.codes, None if saved is None else saved.steps)
