@@ -181,3 +181,23 @@ def stream_ptr():
     import torch
 
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def call(name, device, *args):
+    """lib().<name>(*args, stream) on `device`'s current stream, with `device` current; addresses and sizes are plain integers (None: NULL).  The form of
+    small operators that are called from user code, where the host's time is the call's: no context manager and no stream object on the usual path."""
+    import torch
+
+    index = device.index
+    if torch.cuda.current_device() == index:
+        check(getattr(_lib or lib(), name)(*args, _raw_stream(index)), name)
+    else:
+        with torch.cuda.device(index):
+            check(getattr(_lib or lib(), name)(*args, _raw_stream(index)), name)
+
+
+def _raw_stream(index):
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream

@@ -1589,6 +1589,8 @@ def _type_of(t, who):
 
 def _rows_of(t, who):
     """t as rows of consecutive elements: (2-D tensor, row stride); a view wherever the strides allow it."""
+    if t.dim() == 2 and t.is_contiguous() and t.numel() > 0:
+        return t, t.shape[1]
     if t.dim() == 0:
         raise ValueError(f"{who}: needs at least one dimension")
     cols = t.shape[-1]
@@ -1611,10 +1613,10 @@ def _once(who):
         raise RuntimeError(f"{who}: the backward pass is not differentiable (create_graph=True)")
 
 
-def _same_device(who, *tensors):
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) > 1:
-        raise ValueError(f"{who}: tensors on different devices: {sorted(map(str, devs))}")
+def _same_device(who, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{who}: tensors on different devices: {first.device} and {t.device}")
 
 
 class Checkpoint8:
@@ -1662,9 +1664,7 @@ class Checkpoint8:
             raise ValueError("Checkpoint8.restore: needs tensors on the GPU (the kernels have no CPU form)")
         dev = self.codes.device
         out = torch.empty(self.shape, dtype=dtype, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().spf_saved8_restore(_lib.ptr(self.codes), _lib.ptr(self.steps), self.rows, self.cols, _lib.ptr(out), _TYPES[dtype], self.cols,
-                                                     _lib.stream_ptr()), "spf_saved8_restore")
+        _lib.call("spf_saved8_restore", dev, self.codes.data_ptr(), self.steps.data_ptr(), self.codes.shape[0], self.cols, out.data_ptr(), _TYPES[dtype], self.cols)
         return out
 
 
@@ -1678,43 +1678,69 @@ def checkpoint8(x) -> Checkpoint8:
     code = _type_of(x, "checkpoint8")
     m, ld = _rows_of(x.detach(), "checkpoint8")
     codes, steps = _empty8(m.shape[0], m.shape[1], x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().spf_saved8_pack(_lib.ptr(m), code, ld, m.shape[0], m.shape[1], _lib.ptr(codes), _lib.ptr(steps), _lib.stream_ptr()), "spf_saved8_pack")
+    _lib.call("spf_saved8_pack", x.device, m.data_ptr(), code, ld, m.shape[0], m.shape[1], codes.data_ptr(), steps.data_ptr())
     return Checkpoint8(codes, steps, m.shape[1], x.dtype, x.shape)
 
 
-class _Act8(_GradModeFunction):
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _bytes8(rows, cols):
+    """(bytes of the codes, bytes in all) of an 8-bit form that is kept as one buffer: codes, then steps."""
+    blocks = -(-cols // 32)
+    return rows * blocks * 32, rows * blocks * 33
+
+
+def _needs_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _act8_forward(x, kind, param, train, out8):
+    """-> y, what the backward pass reads (one buffer; None unless train), codes and steps of y (None unless out8)"""
+    m, ld = _rows_of(x, "act8")
+    rows, cols = m.shape
+    y = x.new_empty(x.shape)
+    kept = codes = steps = None
+    at_in = at_out = (None, None)
+    by_output = kind == _ACTS["leaky_relu"][0]                # the sign of y is the sign of x: one 8-bit form serves both this layer and the next
+    if out8:
+        codes, steps = _empty8(rows, cols, x.device)
+        at_out = codes.data_ptr(), steps.data_ptr()
+    if train and not (by_output and out8):
+        n, total = _bytes8(rows, cols)
+        kept = torch.empty(total, dtype=torch.uint8, device=x.device)
+        at = kept.data_ptr(), kept.data_ptr() + n
+        at_in, at_out = (at_in, at) if by_output else (at, at_out)
+    _lib.call("spf_act8_forward", x.device, m.data_ptr(), _TYPES[x.dtype], ld, rows, cols, kind, param, y.data_ptr(), cols, *at_in, *at_out)
+    return y, kept, codes, steps
+
+
+class _Act8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kind, param, out8):
-        code = _TYPES[x.dtype]
-        m, ld = _rows_of(x, "act8")
-        rows, cols = m.shape
-        dev = x.device
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        train = _GradModeFunction._outer_grad_mode and ctx.needs_input_grad[0]
-        by_output = kind == _ACTS["leaky_relu"][0]            # the sign of y is the sign of x: one 8-bit form serves both this layer and the next
-        in8 = _empty8(rows, cols, dev) if train and not by_output else (None, None)
-        o8 = _empty8(rows, cols, dev) if out8 or (train and by_output) else (None, None)
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().spf_act8_forward(_lib.ptr(m), code, ld, rows, cols, kind, param, _lib.ptr(y), cols, *[_lib.ptr(t) for t in in8 + o8],
-                                                   _lib.stream_ptr()), "spf_act8_forward")
-        if train:
-            ctx.save_for_backward(*(o8 if by_output else in8))
-            ctx.kind, ctx.param = kind, param
+        y, kept, codes, steps = _act8_forward(x, kind, param, True, out8)
+        ctx.save_for_backward(*((codes, steps) if kept is None else (kept,)))
+        ctx.kind, ctx.param = kind, param
         if not out8:
             return y
-        ctx.mark_non_differentiable(*o8)
-        return (y,) + o8
+        ctx.mark_non_differentiable(codes, steps)
+        return y, codes, steps
 
     @staticmethod
     def backward(ctx, g, *_):
         _once("act8")
-        codes, steps = ctx.saved_tensors
-        dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        saved = ctx.saved_tensors
         m, ld = _rows_of(g, "act8")
-        with torch.cuda.device(g.device):
-            _lib.check(_lib.lib().spf_act8_backward(_lib.ptr(m), _TYPES[g.dtype], ld, m.shape[0], m.shape[1], ctx.kind, ctx.param, _lib.ptr(codes), _lib.ptr(steps),
-                                                    _lib.ptr(dx), m.shape[1], _lib.stream_ptr()), "spf_act8_backward")
+        rows, cols = m.shape
+        dx = g.new_empty(g.shape)
+        codes = saved[0].data_ptr()
+        steps = saved[1].data_ptr() if len(saved) == 2 else codes + _bytes8(rows, cols)[0]
+        _lib.call("spf_act8_backward", g.device, m.data_ptr(), _TYPES[g.dtype], ld, rows, cols, ctx.kind, ctx.param, codes, steps, dx.data_ptr(), cols)
         return dx, None, None, None
 
 
@@ -1735,60 +1761,89 @@ def act8(x, kind, param=None, out8=False):
         raise ValueError("act8: softplus needs beta > 0")
     if x.dim() == 0:
         raise ValueError("act8: needs at least one dimension")
-    if not out8:
-        return _Act8.apply(x, number, param, False)
-    y, codes, steps = _Act8.apply(x, number, param, True)
+    if _needs_grad(x):
+        r = _Act8.apply(x, number, param, bool(out8))
+        if not out8:
+            return r
+        y, codes, steps = r
+    else:
+        y, _, codes, steps = _act8_forward(x, number, param, False, out8)
+        if not out8:
+            return y
     return y, Checkpoint8(codes, steps, x.shape[-1], x.dtype, x.shape)
 
 
-class _LayerNorm(_GradModeFunction):
+def _sinks_of(needs, *params):
+    """The gradient sinks of the parameters that need a gradient, if all of those have one (else None)."""
+    sinks = [_sink(t) if need and t is not None else None for t, need in zip(params, needs)]
+    return sinks if any(s is not None for s in sinks) and all(s is not None or not need for s, need in zip(sinks, needs)) else None
+
+
+def _layer_norm_forward(x, w, b, eps, train, saved8, out8):
+    """-> y, the rows used (x itself, or the copy of it that its strides called for), [mean, rstd] (None unless train), x in 8 bits as one buffer (None unless
+    train and saved8), codes and steps of y (None unless out8)"""
+    m, ld = _rows_of(x, "layer_norm")
+    rows, cols = m.shape
+    dev = x.device
+    y = x.new_empty(x.shape)
+    stat = kept = codes = steps = None
+    at_in = at_out = at_stat = (None, None)
+    if out8:
+        codes, steps = _empty8(rows, cols, dev)
+        at_out = codes.data_ptr(), steps.data_ptr()
+    if train:
+        stat = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+        at_stat = stat.data_ptr(), stat.data_ptr() + 4 * rows
+        if saved8:
+            n, total = _bytes8(rows, cols)
+            kept = torch.empty(total, dtype=torch.uint8, device=dev)
+            at_in = kept.data_ptr(), kept.data_ptr() + n
+    wtype = _TYPES[(x if w is None and b is None else b if w is None else w).dtype]
+    _lib.call("spf_layer_norm_forward", dev, m.data_ptr(), _TYPES[x.dtype], ld, rows, cols, _address(w), _address(b), wtype, eps, y.data_ptr(), cols, *at_stat, *at_in,
+              *at_out)
+    return y, (x if m.data_ptr() == x.data_ptr() else m), stat, kept, codes, steps
+
+
+class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, eps, saved8, out8):
-        code = _TYPES[x.dtype]
-        m, ld = _rows_of(x, "layer_norm")
-        rows, cols = m.shape
-        dev = x.device
-        wtype = _TYPES[(w if w is not None else b if b is not None else x).dtype]
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        train = _GradModeFunction._outer_grad_mode and any(ctx.needs_input_grad[:3])
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=dev) if train else (None, None)
-        in8 = _empty8(rows, cols, dev) if train and saved8 else (None, None)
-        o8 = _empty8(rows, cols, dev) if out8 else (None, None)
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().spf_layer_norm_forward(_lib.ptr(m), code, ld, rows, cols, _lib.ptr(w), _lib.ptr(b), wtype, eps, _lib.ptr(y), cols, _lib.ptr(mean),
-                                                         _lib.ptr(rstd), *[_lib.ptr(t) for t in in8 + o8], _lib.stream_ptr()), "spf_layer_norm_forward")
-        if train:
-            keep_x = None if saved8 else (x if m.data_ptr() == x.data_ptr() else m)
-            ctx.save_for_backward(keep_x, mean, rstd, w, *in8)
-            ctx.wtype, ctx.bias = wtype, b is not None
-            sinks = [_sink(t) if t is not None and need else None for t, need in zip((w, b), ctx.needs_input_grad[1:3])]
-            needed = [s for s, need in zip(sinks, ctx.needs_input_grad[1:3]) if need]
-            ctx.sinks = sinks if needed and all(s is not None for s in needed) else None
+        y, used, stat, kept, codes, steps = _layer_norm_forward(x, w, b, eps, True, saved8, out8)
+        ctx.save_for_backward(None if saved8 else used, stat, kept, w)
+        ctx.wdtype = (x if w is None and b is None else b if w is None else w).dtype
+        ctx.sinks = _sinks_of(ctx.needs_input_grad[1:3], w, b)
         if not out8:
             return y
-        ctx.mark_non_differentiable(*o8)
-        return (y,) + o8
+        ctx.mark_non_differentiable(codes, steps)
+        return y, codes, steps
 
     @staticmethod
     def backward(ctx, g, *_):
         _once("layer_norm")
-        x, mean, rstd, w, codes, steps = ctx.saved_tensors
+        x, stat, kept, w = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = g.device
         m, ld = _rows_of(g, "layer_norm")
         rows, cols = m.shape
-        mx, ldx = (None, 0) if x is None else _rows_of(x, "layer_norm")
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(g.shape, dtype=g.dtype, device=dev) if need_x else None
-        wdtype = {v: k for k, v in _TYPES.items()}[ctx.wtype]
-        new = torch.zeros if rows == 0 else torch.empty
-        dw, db = ctx.sinks if ctx.sinks is not None else [new((cols,), dtype=wdtype, device=dev) if need else None for need in (need_w, need_b)]
-        with torch.cuda.device(dev):
-            l = _lib.lib()
-            ws = torch.empty((int(l.spf_layer_norm_workspace_floats(rows, cols)),), dtype=torch.float32, device=dev) if need_w or need_b else None
-            _lib.check(l.spf_layer_norm_backward(_lib.ptr(m), _TYPES[g.dtype], ld, rows, cols, _lib.ptr(mx), ldx, _lib.ptr(codes), _lib.ptr(steps), _lib.ptr(mean),
-                                                 _lib.ptr(rstd), _lib.ptr(w), ctx.wtype, _lib.ptr(dx), cols, _lib.ptr(dw), _lib.ptr(db),
-                                                 int(ctx.sinks is not None), _lib.ptr(ws), _lib.stream_ptr()), "spf_layer_norm_backward")
-        return (dx,) + ((None, None) if ctx.sinks is not None else (dw, db)) + (None, None, None)
+        mx, ldx, at_kept = None, 0, (None, None)
+        if kept is None:
+            mx, ldx = _rows_of(x, "layer_norm")
+        else:
+            at_kept = kept.data_ptr(), kept.data_ptr() + _bytes8(rows, cols)[0]
+        dx = g.new_empty(g.shape) if need_x else None
+        ws = None
+        dw, db = ctx.sinks if ctx.sinks is not None else (None, None)
+        if need_w or need_b:
+            ws = torch.empty(_lib.lib().spf_layer_norm_workspace_floats(rows, cols), dtype=torch.float32, device=dev)
+            if ctx.sinks is None:
+                new = torch.zeros if rows == 0 else torch.empty
+                dw = new(cols, dtype=ctx.wdtype, device=dev) if need_w else None
+                db = new(cols, dtype=ctx.wdtype, device=dev) if need_b else None
+        at_stat = stat.data_ptr()
+        _lib.call("spf_layer_norm_backward", dev, m.data_ptr(), _TYPES[g.dtype], ld, rows, cols, _address(mx), ldx, *at_kept, at_stat, at_stat + 4 * rows, _address(w),
+                  _TYPES[ctx.wdtype], _address(dx), cols, _address(dw), _address(db), int(ctx.sinks is not None), _address(ws))
+        if ctx.sinks is not None:
+            dw = db = None
+        return dx, dw, db, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
@@ -1808,20 +1863,23 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError("layer_norm: eps must be finite and not negative")
-    if not out8:
-        return _LayerNorm.apply(x, weight, bias, eps, bool(saved8), False)
-    y, codes, steps = _LayerNorm.apply(x, weight, bias, eps, bool(saved8), True)
+    if _needs_grad(x, weight, bias):
+        r = _LayerNorm.apply(x, weight, bias, eps, bool(saved8), bool(out8))
+        if not out8:
+            return r
+        y, codes, steps = r
+    else:
+        y, _, _, _, codes, steps = _layer_norm_forward(x, weight, bias, eps, False, False, out8)
+        if not out8:
+            return y
     return y, Checkpoint8(codes, steps, x.shape[-1], x.dtype, x.shape)
 
 
 def _wgrad8_into(m, ld, codes, steps, cols, dw, db, accumulate):
     rows, n = m.shape
-    dev = m.device
-    with torch.cuda.device(dev):
-        l = _lib.lib()
-        ws = torch.empty((int(l.spf_wgrad8_workspace_floats(rows, n, cols)),), dtype=torch.float32, device=dev)
-        _lib.check(l.spf_wgrad8(_lib.ptr(m), _TYPES[m.dtype], ld, _lib.ptr(codes), _lib.ptr(steps), rows, n, cols, _lib.ptr(dw), _lib.ptr(db), _TYPES[dw.dtype],
-                                int(accumulate), _lib.ptr(ws), _lib.stream_ptr()), "spf_wgrad8")
+    ws = torch.empty(_lib.lib().spf_wgrad8_workspace_floats(rows, n, cols), dtype=torch.float32, device=m.device)
+    _lib.call("spf_wgrad8", m.device, m.data_ptr(), _TYPES[m.dtype], ld, codes.data_ptr(), steps.data_ptr(), rows, n, cols, dw.data_ptr(), _address(db),
+              _TYPES[dw.dtype], int(accumulate), ws.data_ptr())
 
 
 def wgrad8(g, saved, out=None, dbias=None, bias=True):
@@ -1854,18 +1912,15 @@ def wgrad8(g, saved, out=None, dbias=None, bias=True):
     return dw, db
 
 
-class _Linear8(_GradModeFunction):
+class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, codes, steps):
         y = torch.nn.functional.linear(x, w, b)               # a plain product: the library's
-        if _GradModeFunction._outer_grad_mode and any(ctx.needs_input_grad[:3]):
-            if codes is None and any(ctx.needs_input_grad[1:3]):
-                ck = checkpoint8(x)
-                codes, steps = ck.codes, ck.steps
-            ctx.save_for_backward(w, codes, steps)
-            sinks = [_sink(t) if t is not None and need else None for t, need in zip((w, b), ctx.needs_input_grad[1:3])]
-            needed = [s for s, need in zip(sinks, ctx.needs_input_grad[1:3]) if need]
-            ctx.sinks = sinks if ctx.needs_input_grad[1] and all(s is not None for s in needed) else None
+        if codes is None and any(ctx.needs_input_grad[1:3]):
+            ck = checkpoint8(x)
+            codes, steps = ck.codes, ck.steps
+        ctx.save_for_backward(w, codes, steps)
+        ctx.sinks = _sinks_of(ctx.needs_input_grad[1:3], w, b) if ctx.needs_input_grad[1] else None
         return y
 
     @staticmethod
@@ -1905,4 +1960,6 @@ def linear8(x, weight, bias=None, saved=None):
             rows *= k
         if not isinstance(saved, Checkpoint8) or saved.rows != rows or saved.cols != x.shape[-1]:
             raise ValueError("linear8: saved must be the Checkpoint8 of x")
+    if not _needs_grad(x, weight, bias):
+        return torch.nn.functional.linear(x, weight, bias)
     return _Linear8.apply(x, weight, bias, None if saved is None else saved.codes, None if saved is None else saved.steps)
