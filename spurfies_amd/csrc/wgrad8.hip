@@ -31,7 +31,8 @@ struct wgrad8_args {
     long long rows, share;           // rows in all, and of one split (a multiple of the stage)
     int n, k, nb;                    // columns of G, columns of A, 32-column blocks of a row of A
     int tiles_n, tiles_k, splits;
-    float *dw, *db;                  // fp32 tiles: [split][n][k], [split][n] (db: null or)
+    void *dw, *db;                   // splits == 1: the results; else fp32 tiles [split][n][k], [split][n].  db: null or
+    int type, add;                   // of the results (splits == 1)
 };
 
 // the high halves of two floats as one word: two bf16 by truncation
@@ -53,32 +54,42 @@ __device__ __forceinline__ bf16x8 read_columns(const __bf16* p, int pitch) {
     return r.v;
 }
 
+template <typename W> __device__ __forceinline__ void put(void* out, size_t i, float v, bool add) {
+    W* p = reinterpret_cast<W*>(out) + i;
+    *p = (W)(add ? (float)*p + v : v);
+}
+
 template <typename T, int TN, int TK, int WN, int WK, int MS>
 __global__ void __launch_bounds__(64 * WN * WK)
 wgrad8_kernel(wgrad8_args a) {
     constexpr int THREADS = 64 * WN * WK, NP = PIECES<T>, FN = TN / WN / 32, FK = TK / WK / 32;
     constexpr int PN = TN + 32, PK = TK + 32;                              // row pitches in LDS, elements
     constexpr int GC = MS * TN / 8 / THREADS, GROW = THREADS / (TN / 8);     // 8-element pieces of G a thread loads, and the rows between them
-    constexpr int AC = MS * TK / 16 / THREADS, AROW = THREADS / (TK / 16);   // 16-byte pieces of A
+    constexpr int AB = MS * TK / 16 >= THREADS ? 16 : 8;                    // bytes of A in a piece
+    constexpr int AC = MS * TK / AB / THREADS, AROW = THREADS / (TK / AB);
     static_assert(GC >= 1 && AC >= 1 && GC * GROW == MS && AC * AROW == MS, "the loads cover a stage");
     __shared__ __attribute__((aligned(16))) __bf16 sg[2][NP][MS * PN];
     __shared__ __attribute__((aligned(16))) __bf16 sa[2][MS * PK];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int split = blockIdx.x / (a.tiles_n * a.tiles_k), tile = blockIdx.x % (a.tiles_n * a.tiles_k);
-    const int n0 = (tile / a.tiles_k) * TN, k0 = (tile % a.tiles_k) * TK;
+    // Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles, so that the ones that share rows and columns meet in its L2: split by split, and
+    // within a split strips of eight tiles of G's columns.
+    const int tiles = a.tiles_n * a.tiles_k, total = tiles * a.splits;
+    const int wg = total % 8 == 0 ? (int)(blockIdx.x % 8) * (total / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+    const int split = wg / tiles, tile = wg % tiles, strip = tile / (8 * a.tiles_k);
+    const int height = min(8, a.tiles_n - 8 * strip), in_strip = tile - strip * 8 * a.tiles_k;
+    const int n0 = (8 * strip + in_strip % height) * TN, k0 = (in_strip / height) * TK;
     const long long m_begin = split * a.share, m_end = min(m_begin + a.share, a.rows);
 
     // this thread's pieces of a stage
-    const int gcol = (tid % (TN / 8)) * 8, grow = tid / (TN / 8), acol = (tid % (TK / 16)) * 16, arow = tid / (TK / 16);
+    const int gcol = (tid % (TN / 8)) * 8, grow = tid / (TN / 8), acol = (tid % (TK / AB)) * AB, arow = tid / (TK / AB);
     const T* gp = (const T*)a.g + n0 + gcol;
     const int g_left = a.n - n0 - gcol;
     const bool a_in = k0 + acol < a.nb * S8_BLOCK;
     const uint8_t* ap = a.codes + k0 + acol;
     const uint8_t* ep = a.steps + (k0 + acol) / S8_BLOCK;
     vec_t<T> rg[GC][8 / VEC<T>];
-    u32x4 ra[AC];
-    uint32_t re[AC];
+    uint32_t ra[AC][AB / 4], re[AC];
     auto load = [&](long long m0) {
 #pragma unroll
         for (int i = 0; i < GC; ++i) {
@@ -90,106 +101,146 @@ wgrad8_kernel(wgrad8_args a) {
 #pragma unroll
         for (int i = 0; i < AC; ++i) {
             const long long m = m0 + arow + i * AROW;
-            ra[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < AB / 4; ++j) ra[i][j] = 0;
             re[i] = 0;
             if (a_in && m < m_end) {
-                ra[i] = *reinterpret_cast<const u32x4*>(ap + m * a.nb * S8_BLOCK);
+                const uint8_t* p = ap + m * a.nb * S8_BLOCK;
+                if constexpr (AB == 16) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) ra[i][j] = v[j];
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p);
+                    ra[i][0] = v.x, ra[i][1] = v.y;
+                }
                 re[i] = ep[m * a.nb];
             }
         }
     };
     float bias[8] = {};
     const bool with_bias = a.db && k0 == 0;
-    auto store = [&](int buf) {
+    auto store_g = [&](int buf, int i) {
+        float f[8];
 #pragma unroll
-        for (int i = 0; i < GC; ++i) {
-            float f[8];
+        for (int j = 0; j < 8; ++j) f[j] = (float)rg[i][j / VEC<T>][j % VEC<T>];
+        if (with_bias)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = (float)rg[i][j / VEC<T>][j % VEC<T>];
-            if (with_bias)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) bias[j] += f[j];
+            for (int j = 0; j < 8; ++j) bias[j] += f[j];
+        __bf16* d = &sg[buf][0][(grow + i * GROW) * PN + gcol];
+        if constexpr (NP == 1) {
+            *reinterpret_cast<vec_t<T>*>(d) = rg[i][0];
+        } else {
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
                 u32x4 w;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = high_halves(f[2 * j], f[2 * j + 1]);
-                *reinterpret_cast<u32x4*>(&sg[buf][p][(grow + i * GROW) * PN + gcol]) = w;
+                *reinterpret_cast<u32x4*>(d + p * MS * PN) = w;
                 if (p + 1 < NP)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) f[j] -= high_part(f[j]);
             }
         }
+    };
+    auto store_a = [&](int buf, int i) {
+        const float step = s8_step(re[i]);
+        __bf16* d = &sa[buf][(arow + i * AROW) * PK + acol];
 #pragma unroll
-        for (int i = 0; i < AC; ++i) {
-            const float step = s8_step(re[i]);
-            u32x4 w[2];
+        for (int h = 0; h < AB / 8; ++h) {
+            u32x4 w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t c = ra[i][j], mag = c & 0x7f7f7f7fu;
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t c = ra[i][2 * h + j], mag = c & 0x7f7f7f7fu;
                 const float m0 = (float)(mag & 0xffu) * step, m1 = (float)((mag >> 8) & 0xffu) * step, m2 = (float)((mag >> 16) & 0xffu) * step, m3 = (float)(mag >> 24) * step;
                 // the signs: bytes 0, 1 and 2, 3 moved to the tops of two bf16 pairs
-                w[j / 2][2 * (j % 2)] = high_halves(m0, m1) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
-                w[j / 2][2 * (j % 2) + 1] = high_halves(m2, m3) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
+                w[2 * j] = high_halves(m0, m1) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
+                w[2 * j + 1] = high_halves(m2, m3) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
             }
-            __bf16* d = &sa[buf][(arow + i * AROW) * PK + acol];
-            *reinterpret_cast<u32x4*>(d) = w[0];
-            *reinterpret_cast<u32x4*>(d + 8) = w[1];
+            *reinterpret_cast<u32x4*>(d + 8 * h) = w;
         }
     };
 
     f32x16 acc[FN][FK] = {};
     const int wn = (wave / WK) * (TN / WN), wk = (wave % WK) * (TK / WK);
     const int at_row = (lane >> 5) * 8 + ((lane >> 2) & 3), at_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    auto multiply = [&](int buf, int s) {
+        bf16x8 fa[FK];
+#pragma unroll
+        for (int j = 0; j < FK; ++j) fa[j] = read_columns(&sa[buf][(16 * s + at_row) * PK + wk + 32 * j + at_col], PK);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const bf16x8 fg = read_columns(&sg[buf][p][(16 * s + at_row) * PN + wn + 32 * i + at_col], PN);
+#pragma unroll
+                for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg, fa[j], acc[i][j], 0, 0, 0);
+            }
+    };
 
-    if (m_begin < m_end) load(m_begin);
+    // Stage i is multiplied while stage i + 1 goes from registers to the other LDS buffer, a part behind each 16 rows, and stage i + 2 is under way from memory.
+    if (m_begin < m_end) {
+        load(m_begin);
+#pragma unroll
+        for (int i = 0; i < GC; ++i) store_g(0, i);
+#pragma unroll
+        for (int i = 0; i < AC; ++i) store_a(0, i);
+        load(m_begin + MS);                                                 // (rows behind the share's end are zeros)
+        lds_barrier();
+    }
     int buf = 0;
     for (long long m0 = m_begin; m0 < m_end; m0 += MS, buf ^= 1) {
-        store(buf);
-        if (m0 + MS < m_end) load(m0 + MS);
-        lds_barrier();
+        constexpr int PARTS = MS / 16;
 #pragma unroll
-        for (int s = 0; s < MS / 16; ++s) {
-            bf16x8 fa[FK];
+        for (int s = 0; s < PARTS; ++s) {
+            multiply(buf, s);
 #pragma unroll
-            for (int j = 0; j < FK; ++j) fa[j] = read_columns(&sa[buf][(16 * s + at_row) * PK + wk + 32 * j + at_col], PK);
+            for (int i = 0; i < GC; ++i)
+                if (i * PARTS / GC == s) store_g(buf ^ 1, i);
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-#pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    const bf16x8 fg = read_columns(&sg[buf][p][(16 * s + at_row) * PN + wn + 32 * i + at_col], PN);
-#pragma unroll
-                    for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg, fa[j], acc[i][j], 0, 0, 0);
-                }
+            for (int i = 0; i < AC; ++i)
+                if ((AC - 1 - i) * PARTS / AC == PARTS - 1 - s) store_a(buf ^ 1, i);
         }
+        load(m0 + 2 * MS);
+        lds_barrier();
     }
 
     // the tile: a lane holds column (lane & 31) and rows 8 (q / 4) + 4 (lane / 32) + q % 4 of each 32 x 32 block
-    float* dw = a.dw + (size_t)split * a.n * a.k;
+    auto write = [&](auto one, void* dw, void* db, bool add) {
+        using W = decltype(one);
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+        for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int j = 0; j < FK; ++j) {
-            const int col = k0 + wk + 32 * j + (lane & 31);
+            for (int j = 0; j < FK; ++j) {
+                const int col = k0 + wk + 32 * j + (lane & 31);
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int row = n0 + wn + 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4;
-                if (row < a.n && col < a.k) dw[(size_t)row * a.k + col] = acc[i][j][q];
+                for (int q = 0; q < 16; ++q) {
+                    const int row = n0 + wn + 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4;
+                    if (row < a.n && col < a.k) put<W>(dw, (size_t)row * a.k + col, acc[i][j][q], add);
+                }
+            }
+        if (with_bias) {                                                    // the same for the whole workgroup
+            __syncthreads();
+            float* fold = reinterpret_cast<float*>(&sg[0][0][0]);           // [GROW][TN]
+            static_assert(GROW * TN * 4 <= (int)sizeof(sg), "the column sums fit");
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fold[grow * TN + gcol + j] = bias[j];
+            __syncthreads();
+            for (int c = tid; c < TN; c += THREADS) {
+                float s = 0.f;
+                for (int r = 0; r < GROW; ++r) s += fold[r * TN + c];
+                if (n0 + c < a.n) put<W>(db, n0 + c, s, add);
             }
         }
-    if (with_bias) {                                                        // the same for the whole workgroup
-        __syncthreads();
-        float* fold = reinterpret_cast<float*>(&sg[0][0][0]);               // [GROW][TN]
-        static_assert(GROW * TN * 4 <= (int)sizeof(sg), "the column sums fit");
-#pragma unroll
-        for (int j = 0; j < 8; ++j) fold[grow * TN + gcol + j] = bias[j];
-        __syncthreads();
-        for (int c = tid; c < TN; c += THREADS) {
-            float s = 0.f;
-            for (int r = 0; r < GROW; ++r) s += fold[r * TN + c];
-            if (n0 + c < a.n) a.db[(size_t)split * a.n + n0 + c] = s;
-        }
-    }
+    };
+    if (a.splits > 1)
+        write(float(), (float*)a.dw + (size_t)split * a.n * a.k, (float*)a.db + (size_t)split * a.n, false);
+    else if (a.type == SPF_TYPE_F32)
+        write(float(), a.dw, a.db, a.add != 0);
+    else if (a.type == SPF_TYPE_BF16)
+        write(__bf16(), a.dw, a.db, a.add != 0);
+    else
+        write(_Float16(), a.dw, a.db, a.add != 0);
 }
 
 // out[i] (+)= sum over the splits, in order; eight threads an element group share the splits
@@ -218,34 +269,36 @@ wgrad8_reduce_kernel(const float* __restrict__ tiles, int splits, long long coun
 }
 
 struct plan {
-    int tn, tk, ms, tiles_n, tiles_k, splits;
+    int tn, tk, tiles_n, tiles_k, splits;
     int64_t share;
 };
-// A 256 x 256 tile reads each operand least often and keeps the matrix pipe fed; a layer that does not fill one takes 64 x 64.  The rows are split until
-// there is a workgroup for each of the 256 compute units, as long as a share is worth its fp32 tile (eight stages).
+constexpr int STAGE = 32;
+// A 256 x 256 tile reads each operand least often and keeps the matrix pipe fed, but a workgroup has a compute unit to itself and leaves 256 KB behind:
+// it is taken where every compute unit gets eight stages of rows or more.  Smaller work takes 64 x 64 tiles, several to a compute unit, and shares as short
+// as two stages, since what counts there is the chain of loads.
 plan plan_of(int64_t rows, int64_t n, int64_t k) {
     plan p;
-    const bool big = n > 128 && k > 128;
+    const int64_t stages = (rows + STAGE - 1) / STAGE;
+    const bool big = n > 128 && k > 128 && ((n + 255) / 256) * ((k + 255) / 256) * stages >= 256 * 8;
     p.tn = p.tk = big ? 256 : 64;
-    p.ms = big ? 32 : 64;
     p.tiles_n = (int)((n + p.tn - 1) / p.tn);
     p.tiles_k = (int)((k + p.tk - 1) / p.tk);
-    const int64_t stages = (rows + p.ms - 1) / p.ms, tiles = (int64_t)p.tiles_n * p.tiles_k;
-    int64_t s = (big ? 256 : 1024) / tiles;
-    s = s < stages / 8 ? s : stages / 8;
+    const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, most = big ? 256 : 1024, least = big ? 8 : 2;
+    int64_t s = most / tiles;
+    s = s < stages / least ? s : stages / least;
     s = s < 1 ? 1 : s;
     const int64_t per = (stages + s - 1) / s;
     p.splits = (int)((stages + per - 1) / per);
-    p.share = per * p.ms;
+    p.share = per * STAGE;
     return p;
 }
 
 template <typename T> void launch(const wgrad8_args& a, const plan& p, hipStream_t s) {
     const unsigned wgs = (unsigned)(p.tiles_n * p.tiles_k * p.splits);
     if (p.tn == 256)
-        wgrad8_kernel<T, 256, 256, 2, 4, 32><<<wgs, 512, 0, s>>>(a);
+        wgrad8_kernel<T, 256, 256, 2, 4, STAGE><<<wgs, 512, 0, s>>>(a);
     else
-        wgrad8_kernel<T, 64, 64, 2, 2, 64><<<wgs, 256, 0, s>>>(a);
+        wgrad8_kernel<T, 64, 64, 2, 2, STAGE><<<wgs, 256, 0, s>>>(a);
 }
 
 const char* bad_sizes(int64_t rows, int64_t n, int64_t k) {
@@ -261,7 +314,8 @@ extern "C" {
 
 int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols) {
     if (bad_sizes(rows, n, cols) || rows == 0 || n == 0 || cols == 0) return 0;
-    return (int64_t)plan_of(rows, n, cols).splits * n * (cols + 1);
+    const int64_t splits = plan_of(rows, n, cols).splits;
+    return splits > 1 ? splits * n * (cols + 1) : 0;
 }
 
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols, void* dw, void* db,
@@ -270,22 +324,25 @@ int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, c
     if (!type_ok(type) || !type_ok(wtype)) return fail(SPF_EINVAL, "%s: unknown element type", who);
     if (const char* why = bad_sizes(rows, n, cols)) return fail(SPF_EINVAL, "%s: %s", who, why);
     if (rows == 0 || n == 0 || cols == 0) return SPF_OK;
-    if (!g || !codes || !steps || !dw || !workspace) return fail(SPF_EINVAL, "%s: null pointer", who);
+    const plan p = plan_of(rows, n, cols);
+    if (!g || !codes || !steps || !dw || (p.splits > 1 && !workspace)) return fail(SPF_EINVAL, "%s: null pointer", who);
     if (ldg < 0) return fail(SPF_EINVAL, "%s: row stride", who);
     if (misaligned(g, type_size(type)) || misaligned(codes, 16) || misaligned(dw, type_size(wtype)) || misaligned(db, type_size(wtype)) || misaligned(workspace, 4))
         return fail(SPF_EINVAL, "%s: misaligned pointer", who);
-    const plan p = plan_of(rows, n, cols);
-    wgrad8_args a = {g, ldg, codes, steps, rows, p.share, (int)n, (int)cols, (int)((cols + S8_BLOCK - 1) / S8_BLOCK), p.tiles_n, p.tiles_k, p.splits, workspace,
-                     db ? workspace + (int64_t)p.splits * n * cols : nullptr};
+    float* bias_tiles = db ? workspace + (int64_t)p.splits * n * cols : nullptr;
+    wgrad8_args a = {g, ldg, codes, steps, rows, p.share, (int)n, (int)cols, (int)((cols + S8_BLOCK - 1) / S8_BLOCK), p.tiles_n, p.tiles_k, p.splits, dw, db, wtype, accumulate};
+    if (p.splits > 1) a.dw = workspace, a.db = bias_tiles;
     hipStream_t s = (hipStream_t)stream;
     if (type == SPF_TYPE_F32) launch<float>(a, p, s);
     else if (type == SPF_TYPE_BF16) launch<__bf16>(a, p, s);
     else launch<_Float16>(a, p, s);
-    const int64_t groups = (n * cols + 31) / 32 + (db ? (n + 31) / 32 : 0);
-    const auto reduce = [&](auto* w, auto* b) { wgrad8_reduce_kernel<<<(unsigned)groups, 256, 0, s>>>(workspace, p.splits, n * cols, w, a.db, (int)n, b, accumulate); };
-    if (wtype == SPF_TYPE_F32) reduce((float*)dw, (float*)db);
-    else if (wtype == SPF_TYPE_BF16) reduce((__bf16*)dw, (__bf16*)db);
-    else reduce((_Float16*)dw, (_Float16*)db);
+    if (p.splits > 1) {
+        const int64_t groups = (n * cols + 31) / 32 + (db ? (n + 31) / 32 : 0);
+        const auto reduce = [&](auto* w, auto* b) { wgrad8_reduce_kernel<<<(unsigned)groups, 256, 0, s>>>(workspace, p.splits, n * cols, w, bias_tiles, (int)n, b, accumulate); };
+        if (wtype == SPF_TYPE_F32) reduce((float*)dw, (float*)db);
+        else if (wtype == SPF_TYPE_BF16) reduce((__bf16*)dw, (__bf16*)db);
+        else reduce((_Float16*)dw, (_Float16*)db);
+    }
     SPF_LAUNCH_CHECK(who);
     return SPF_OK;
 }

@@ -370,7 +370,25 @@ def test_wgrad8(dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,n,k", [(1, 3, 5), (64, 70, 96), (97, 256, 256), (130, 300, 131), (900, 64, 64)])
+@pytest.mark.parametrize("rows,n,k", [(66001, 256, 130), (66001, 256, 256), (7400, 520, 515), (3300, 1030, 800)])
+def test_wgrad8_of_large_layers(dtype, rows, n, k):
+    """The wide tiles, with and without split rows and with ragged edges; the restored input is the kernels' own (tested byte for byte above)."""
+    from spurfies_amd import ops
+
+    a, g = randn((rows, k), dtype, 1), randn((rows, n), dtype, 2)
+    ck = ops.checkpoint8(a)
+    dw, db = ops.wgrad8(g, ck)
+    A, G = f64(ck.restore(torch.float32)), f64(g)
+    want = G.T @ A
+    # 2 u sqrt(chain) of sqrt(rows) times the factors' sizes (1 each): the spread of a sum of independent roundings, held to eight of it
+    close(dw, want, 8 * 2 * U * np.sqrt(3 * rows) * np.sqrt(rows) * 2, "dw")
+    close(db, G.sum(axis=0), 8 * U * np.sqrt(rows) * np.sqrt(rows) * 2, "db")
+    assert np.linalg.norm(f64(dw) - want) < 2 * U * 8 * np.sqrt(3 * rows + 64) * np.linalg.norm(want)
+    assert all(torch.equal(p, q) for p, q in zip((dw, db), ops.wgrad8(g, ck)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 3, 5), (64, 70, 96), (97, 256, 256), (130, 300, 131), (900, 64, 64), (800, 2050, 2050)])
 def test_wgrad8_is_exact_for_whole_numbers(dtype, rows, n, k):
     """Inputs with as many digits as their type has and sums that fit 24 bits: nothing may round, so every piece of every gradient has to arrive."""
     from spurfies_amd import ops

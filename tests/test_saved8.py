@@ -66,7 +66,8 @@ def test_library_refuses_bad_arguments(lib):
     assert back(p, p, p) == -22 and "one of" in err()
     assert back(p, None, None) == -22 and "workspace" in err()
     assert lib.spf_wgrad8(p, 0, 32, p, p, 4, 32, 32, p, None, 5, 0, p, None) == -22 and "type" in err()
-    assert lib.spf_wgrad8(p, 0, 32, p, p, 4, 32, 32, p, None, 0, 0, None, None) == -22 and "null" in err()
+    assert lib.spf_wgrad8_workspace_floats(1 << 16, 32, 32) > 0
+    assert lib.spf_wgrad8(p, 0, 32, p, p, 1 << 16, 32, 32, p, None, 0, 0, None, None) == -22 and "null" in err()
     assert lib.spf_wgrad8(p, 0, 32, q, p, 4, 32, 32, p, None, 0, 0, p, None) == -22 and "misaligned" in err()
     assert lib.spf_wgrad8(p, 0, 32, p, p, 4, 1 << 21, 32, p, None, 0, 0, p, None) == -22 and "2^20" in err()
 
