@@ -90,32 +90,28 @@ wgrad8_kernel(wgrad8_args a) {
     const uint8_t* ep = a.steps + (k0 + acol) / S8_BLOCK;
     vec_t<T> rg[GC][8 / VEC<T>];
     uint32_t ra[AC][AB / 4], re[AC];
-    auto load = [&](long long m0) {
+    auto load_g = [&](long long m0, int i) {                              // rows behind the share's end are zeros
+        const long long m = m0 + grow + i * GROW;
+        const int left = m < m_end ? g_left : 0;
 #pragma unroll
-        for (int i = 0; i < GC; ++i) {
-            const long long m = m0 + grow + i * GROW;
-            const int left = m < m_end ? g_left : 0;
+        for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = load_vec(gp + m * a.ldg + q * VEC<T>, left - q * VEC<T>);
+    };
+    auto load_a = [&](long long m0, int i) {
+        const long long m = m0 + arow + i * AROW;
 #pragma unroll
-            for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = load_vec(gp + m * a.ldg + q * VEC<T>, left - q * VEC<T>);
-        }
+        for (int j = 0; j < AB / 4; ++j) ra[i][j] = 0;
+        re[i] = 0;
+        if (a_in && m < m_end) {
+            const uint8_t* p = ap + m * a.nb * S8_BLOCK;
+            if constexpr (AB == 16) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-        for (int i = 0; i < AC; ++i) {
-            const long long m = m0 + arow + i * AROW;
-#pragma unroll
-            for (int j = 0; j < AB / 4; ++j) ra[i][j] = 0;
-            re[i] = 0;
-            if (a_in && m < m_end) {
-                const uint8_t* p = ap + m * a.nb * S8_BLOCK;
-                if constexpr (AB == 16) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) ra[i][j] = v[j];
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(p);
-                    ra[i][0] = v.x, ra[i][1] = v.y;
-                }
-                re[i] = ep[m * a.nb];
+                for (int j = 0; j < 4; ++j) ra[i][j] = v[j];
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                ra[i][0] = v.x, ra[i][1] = v.y;
             }
+            re[i] = ep[m * a.nb];
         }
     };
     float bias[8] = {};
@@ -178,14 +174,17 @@ wgrad8_kernel(wgrad8_args a) {
             }
     };
 
-    // Stage i is multiplied while stage i + 1 goes from registers to the other LDS buffer, a part behind each 16 rows, and stage i + 2 is under way from memory.
+    // Stage i is multiplied while stage i + 1 goes from registers to the other LDS buffer, a piece behind each 16 rows, and each piece of stage i + 2 is under
+    // way from memory as soon as its registers are free: for a whole stage's time.
     if (m_begin < m_end) {
-        load(m_begin);
 #pragma unroll
-        for (int i = 0; i < GC; ++i) store_g(0, i);
+        for (int i = 0; i < GC; ++i) load_g(m_begin, i);
 #pragma unroll
-        for (int i = 0; i < AC; ++i) store_a(0, i);
-        load(m_begin + MS);                                                 // (rows behind the share's end are zeros)
+        for (int i = 0; i < AC; ++i) load_a(m_begin, i);
+#pragma unroll
+        for (int i = 0; i < GC; ++i) store_g(0, i), load_g(m_begin + MS, i);
+#pragma unroll
+        for (int i = 0; i < AC; ++i) store_a(0, i), load_a(m_begin + MS, i);
         lds_barrier();
     }
     int buf = 0;
@@ -196,12 +195,11 @@ wgrad8_kernel(wgrad8_args a) {
             multiply(buf, s);
 #pragma unroll
             for (int i = 0; i < GC; ++i)
-                if (i * PARTS / GC == s) store_g(buf ^ 1, i);
+                if (i * PARTS / GC == s) store_g(buf ^ 1, i), load_g(m0 + 2 * MS, i);
 #pragma unroll
             for (int i = 0; i < AC; ++i)
-                if ((AC - 1 - i) * PARTS / AC == PARTS - 1 - s) store_a(buf ^ 1, i);
+                if ((AC - 1 - i) * PARTS / AC == PARTS - 1 - s) store_a(buf ^ 1, i), load_a(m0 + 2 * MS, i);
         }
-        load(m0 + 2 * MS);
         lds_barrier();
     }
 
