@@ -31,8 +31,8 @@ struct wgrad8_args {
     long long rows, share;           // rows in all, and of one split (a multiple of the stage)
     int n, k, nb;                    // columns of G, columns of A, 32-column blocks of a row of A
     int tiles_n, tiles_k, splits;
-    void *dw, *db;                   // splits == 1: the results; else fp32 tiles [split][n][k], [split][n].  db: null or
-    int type, add;                   // of the results (splits == 1)
+    void *dw, *db;                   // of type `type`: the results [n][k], [n], or the splits' fp32 tiles [split][n][k], [split][n].  db: null or
+    int type;
 };
 
 // the high halves of two floats as one word: two bf16 by truncation
@@ -54,12 +54,7 @@ __device__ __forceinline__ bf16x8 read_columns(const __bf16* p, int pitch) {
     return r.v;
 }
 
-template <typename W> __device__ __forceinline__ void put(void* out, size_t i, float v, bool add) {
-    W* p = reinterpret_cast<W*>(out) + i;
-    *p = (W)(add ? (float)*p + v : v);
-}
-
-template <typename T, int TN, int TK, int WN, int WK, int MS>
+template <typename T, int TN, int TK, int WN, int WK, int MS, bool PLAIN>
 __global__ void __launch_bounds__(64 * WN * WK)
 wgrad8_kernel(wgrad8_args a) {
     constexpr int THREADS = 64 * WN * WK, NP = PIECES<T>, FN = TN / WN / 32, FK = TK / WK / 32;
@@ -68,8 +63,10 @@ wgrad8_kernel(wgrad8_args a) {
     constexpr int AB = MS * TK / 16 >= THREADS ? 16 : 8;                    // bytes of A in a piece
     constexpr int AC = MS * TK / AB / THREADS, AROW = THREADS / (TK / AB);
     static_assert(GC >= 1 && AC >= 1 && GC * GROW == MS && AC * AROW == MS, "the loads cover a stage");
-    __shared__ __attribute__((aligned(16))) __bf16 sg[2][NP][MS * PN];
-    __shared__ __attribute__((aligned(16))) __bf16 sa[2][MS * PK];
+    // the two buffers are objects of their own, and every access names its own at compile time: reads of one may pass writes of the other
+    __shared__ __attribute__((aligned(16))) __bf16 sg0[NP][MS * PN], sg1[NP][MS * PN], sa0[MS * PK], sa1[MS * PK];
+    auto g_of = [&](auto buf, int p) -> __bf16* { return decltype(buf)::value ? sg1[p] : sg0[p]; };
+    auto a_of = [&](auto buf) -> __bf16* { return decltype(buf)::value ? sa1 : sa0; };
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles, so that the ones that share rows and columns meet in its L2: split by split, and
@@ -81,28 +78,48 @@ wgrad8_kernel(wgrad8_args a) {
     const int n0 = (8 * strip + in_strip % height) * TN, k0 = (in_strip / height) * TK;
     const long long m_begin = split * a.share, m_end = min(m_begin + a.share, a.rows);
 
-    // this thread's pieces of a stage
+    // This thread's pieces of a stage.  PLAIN: loads without conditions, so that the loop is one basic block and its parts can be interleaved.  The rows behind
+    // the share's end read its last row again: their part of A counts as zero, in the product and (as a factor of G's) in the column sums.  Columns behind
+    // the end read other elements of the row and only reach outputs that do not exist; a piece that the end cuts holds the last eight columns instead.
     const int gcol = (tid % (TN / 8)) * 8, grow = tid / (TN / 8), acol = (tid % (TK / AB)) * AB, arow = tid / (TK / AB);
-    const T* gp = (const T*)a.g + n0 + gcol;
     const int g_left = a.n - n0 - gcol;
     const bool a_in = k0 + acol < a.nb * S8_BLOCK;
-    const uint8_t* ap = a.codes + k0 + acol;
-    const uint8_t* ep = a.steps + (k0 + acol) / S8_BLOCK;
+    const int g_at = PLAIN ? min(n0 + gcol, a.n - 8) : n0 + gcol, a_at = PLAIN && !a_in ? 0 : k0 + acol;
+    const long long g_row = a.ldg * (long long)sizeof(T), a_row = (long long)a.nb * S8_BLOCK;      // bytes
     vec_t<T> rg[GC][8 / VEC<T>];
     uint32_t ra[AC][AB / 4], re[AC];
-    auto load_g = [&](long long m0, int i) {                              // rows behind the share's end are zeros
-        const long long m = m0 + grow + i * GROW;
-        const int left = m < m_end ? g_left : 0;
+    const long long m_last = (m_end - 1) / MS * MS;                         // the share's last stage (shares start at multiples of MS)
+    auto load_g = [&](long long m0, int i) {
+        if constexpr (PLAIN) {
+            const long long m = min(m0, m_last);
+            const uint32_t at = min((uint32_t)(grow + i * GROW), (uint32_t)(m_end - 1 - m)) * (uint32_t)g_row + (uint32_t)g_at * (uint32_t)sizeof(T);
+            const T* p = reinterpret_cast<const T*>((const uint8_t*)a.g + m * g_row + at);
 #pragma unroll
-        for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = load_vec(gp + m * a.ldg + q * VEC<T>, left - q * VEC<T>);
+            for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = *reinterpret_cast<const vec_any_t<T>*>(p + q * VEC<T>);
+        } else {
+            const long long m = m0 + grow + i * GROW;
+            const int left = m < m_end ? g_left : 0;
+#pragma unroll
+            for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = load_vec((const T*)a.g + m * a.ldg + g_at + q * VEC<T>, left - q * VEC<T>);
+        }
     };
     auto load_a = [&](long long m0, int i) {
-        const long long m = m0 + arow + i * AROW;
+        long long m = m0 + arow + i * AROW;
+        const bool in = m < m_end;
+        const uint8_t *p, *e;
+        if constexpr (PLAIN) {
+            m = min(m0, m_last);
+            const uint32_t r = min((uint32_t)(arow + i * AROW), (uint32_t)(m_end - 1 - m));
+            p = a.codes + m * a_row + (r * (uint32_t)a_row + (uint32_t)a_at);
+            e = a.steps + m * a.nb + (r * (uint32_t)a.nb + (uint32_t)a_at / S8_BLOCK);
+        } else {
+            p = a.codes + m * a_row + a_at;
+            e = a.steps + m * a.nb + a_at / S8_BLOCK;
 #pragma unroll
-        for (int j = 0; j < AB / 4; ++j) ra[i][j] = 0;
-        re[i] = 0;
-        if (a_in && m < m_end) {
-            const uint8_t* p = ap + m * a.nb * S8_BLOCK;
+            for (int j = 0; j < AB / 4; ++j) ra[i][j] = 0;
+            re[i] = 0;
+        }
+        if (PLAIN || (a_in && in)) {
             if constexpr (AB == 16) {
                 const u32x4 v = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
@@ -111,101 +128,122 @@ wgrad8_kernel(wgrad8_args a) {
                 const uint2 v = *reinterpret_cast<const uint2*>(p);
                 ra[i][0] = v.x, ra[i][1] = v.y;
             }
-            re[i] = ep[m * a.nb];
+            re[i] = *e;
         }
     };
     float bias[8] = {};
     const bool with_bias = a.db && k0 == 0;
-    auto store_g = [&](int buf, int i) {
-        float f[8];
+    // The conversion of the stage from row m0 on into buffer buf, in units of one 16-byte store each: piece p of G's loads i, and eight bytes h of A's loads i
+    float rest[8];                                                          // of G: what the pieces so far leave
+    auto convert_g = [&](auto buf, int i, int p, long long m0, auto sums) {
+        if (p == 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)rg[i][j / VEC<T>][j % VEC<T>];
-        if (with_bias)
+            for (int j = 0; j < 8; ++j) rest[j] = (float)rg[i][j / VEC<T>][j % VEC<T>];
+            if constexpr (decltype(sums)::value) {
+                const float there = m0 + grow + i * GROW < m_end ? 1.f : 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) bias[j] += f[j];
-        __bf16* d = &sg[buf][0][(grow + i * GROW) * PN + gcol];
-        if constexpr (NP == 1) {
-            *reinterpret_cast<vec_t<T>*>(d) = rg[i][0];
-        } else {
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                u32x4 w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = high_halves(f[2 * j], f[2 * j + 1]);
-                *reinterpret_cast<u32x4*>(d + p * MS * PN) = w;
-                if (p + 1 < NP)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] -= high_part(f[j]);
+                for (int j = 0; j < 8; ++j) bias[j] = __builtin_fmaf(rest[j], there, bias[j]);
             }
         }
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = high_halves(rest[2 * j], rest[2 * j + 1]);
+        if constexpr (NP == 1) w = __builtin_bit_cast(u32x4, rg[i][0]);
+        *reinterpret_cast<u32x4*>(g_of(buf, p) + (grow + i * GROW) * PN + gcol) = w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rest[j] -= high_part(rest[j]);
     };
-    auto store_a = [&](int buf, int i) {
-        const float step = s8_step(re[i]);
-        __bf16* d = &sa[buf][(arow + i * AROW) * PK + acol];
+    auto convert_a = [&](auto buf, int i, int h, long long m0) {
+        const float step = m0 + arow + i * AROW < m_end ? s8_step(re[i]) : 0.f;
+        u32x4 w;
 #pragma unroll
-        for (int h = 0; h < AB / 8; ++h) {
-            u32x4 w;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t c = ra[i][2 * h + j], mag = c & 0x7f7f7f7fu;
-                const float m0 = (float)(mag & 0xffu) * step, m1 = (float)((mag >> 8) & 0xffu) * step, m2 = (float)((mag >> 16) & 0xffu) * step, m3 = (float)(mag >> 24) * step;
-                // the signs: bytes 0, 1 and 2, 3 moved to the tops of two bf16 pairs
-                w[2 * j] = high_halves(m0, m1) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
-                w[2 * j + 1] = high_halves(m2, m3) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
-            }
-            *reinterpret_cast<u32x4*>(d + 8 * h) = w;
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t c = ra[i][2 * h + j], mag = c & 0x7f7f7f7fu;
+            const float v0 = (float)(mag & 0xffu) * step, v1 = (float)((mag >> 8) & 0xffu) * step, v2 = (float)((mag >> 16) & 0xffu) * step, v3 = (float)(mag >> 24) * step;
+            // the signs: bytes 0, 1 and 2, 3 moved to the tops of two bf16 pairs
+            w[2 * j] = high_halves(v0, v1) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
+            w[2 * j + 1] = high_halves(v2, v3) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
+        }
+        *reinterpret_cast<u32x4*>(a_of(buf) + (arow + i * AROW) * PK + acol + 8 * h) = w;
+    };
+    // unit u of them, and the load of the stage from row next on as soon as the registers are free
+    constexpr int G_UNITS = GC * NP, UNITS = G_UNITS + AC * (AB / 8);
+    auto convert = [&](auto buf, int u, long long m0, long long next, auto sums) {
+        if (u < G_UNITS) {
+            convert_g(buf, u / NP, u % NP, m0, sums);
+            if (u % NP == 0) load_g(next, u / NP);
+        } else {
+            const int i = (u - G_UNITS) / (AB / 8), h = (u - G_UNITS) % (AB / 8);
+            convert_a(buf, i, h, m0);
+            if (h == AB / 8 - 1) load_a(next, i);
         }
     };
 
     f32x16 acc[FN][FK] = {};
     const int wn = (wave / WK) * (TN / WN), wk = (wave % WK) * (TK / WK);
     const int at_row = (lane >> 5) * 8 + ((lane >> 2) & 3), at_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    auto multiply = [&](int buf, int s) {
-        bf16x8 fa[FK];
+    auto read_a = [&](auto buf, int s, bf16x8 (&fa)[FK]) {
 #pragma unroll
-        for (int j = 0; j < FK; ++j) fa[j] = read_columns(&sa[buf][(16 * s + at_row) * PK + wk + 32 * j + at_col], PK);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const bf16x8 fg = read_columns(&sg[buf][p][(16 * s + at_row) * PN + wn + 32 * i + at_col], PN);
-#pragma unroll
-                for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg, fa[j], acc[i][j], 0, 0, 0);
-            }
+        for (int j = 0; j < FK; ++j) fa[j] = read_columns(a_of(buf) + (16 * s + at_row) * PK + wk + 32 * j + at_col, PK);
+    };
+    auto read_g = [&](auto buf, int f) {
+        const int s = f / (NP * FN), p = f / FN % NP, i = f % FN;
+        return read_columns(g_of(buf, p) + (16 * s + at_row) * PN + wn + 32 * i + at_col, PN);
     };
 
-    // Stage i is multiplied while stage i + 1 goes from registers to the other LDS buffer, a piece behind each 16 rows, and each piece of stage i + 2 is under
-    // way from memory as soon as its registers are free: for a whole stage's time.
-    if (m_begin < m_end) {
+    // Stage i is multiplied while stage i + 1 goes from registers to the other LDS buffer and stage i + 2 is under way from memory: each load has a whole
+    // stage's time.  The products of each fragment of G stand between the read of the next fragment and a unit of the conversion, and stay there: left
+    // to itself the compiler puts all products first, both waves of a SIMD do so at the same time, and either the matrix or the vector pipe rests.
+    using first = std::integral_constant<int, 0>;
+    using second = std::integral_constant<int, 1>;
+    auto work = [&](auto sums) {
 #pragma unroll
         for (int i = 0; i < GC; ++i) load_g(m_begin, i);
 #pragma unroll
         for (int i = 0; i < AC; ++i) load_a(m_begin, i);
 #pragma unroll
-        for (int i = 0; i < GC; ++i) store_g(0, i), load_g(m_begin + MS, i);
-#pragma unroll
-        for (int i = 0; i < AC; ++i) store_a(0, i), load_a(m_begin + MS, i);
+        for (int u = 0; u < UNITS; ++u) convert(first(), u, m_begin, m_begin + MS, sums);
         lds_barrier();
-    }
-    int buf = 0;
-    for (long long m0 = m_begin; m0 < m_end; m0 += MS, buf ^= 1) {
-        constexpr int PARTS = MS / 16;
+        auto stage = [&](auto here, auto there, long long m0) {
+            constexpr int STEPS = MS / 16, PER_STEP = NP * FN, FRAGMENTS = STEPS * PER_STEP;
+            bf16x8 fa[2][FK], fg[2];
+            read_a(here, 0, fa[0]);
+            fg[0] = read_g(here, 0);
 #pragma unroll
-        for (int s = 0; s < PARTS; ++s) {
-            multiply(buf, s);
+            for (int f = 0; f < FRAGMENTS; ++f) {
+                if (f + 1 < FRAGMENTS) fg[(f + 1) % 2] = read_g(here, f + 1);
+                if (f % PER_STEP == PER_STEP - 1 && f + 1 < FRAGMENTS) read_a(here, f / PER_STEP + 1, fa[(f / PER_STEP + 1) % 2]);
 #pragma unroll
-            for (int i = 0; i < GC; ++i)
-                if (i * PARTS / GC == s) store_g(buf ^ 1, i), load_g(m0 + 2 * MS, i);
+                for (int j = 0; j < FK; ++j)
+                    acc[f % FN][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[f % 2], fa[f / PER_STEP % 2][j], acc[f % FN][j], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < AC; ++i)
-                if ((AC - 1 - i) * PARTS / AC == PARTS - 1 - s) store_a(buf ^ 1, i), load_a(m0 + 2 * MS, i);
+                for (int u = 0; u < UNITS; ++u)
+                    if (u * FRAGMENTS / UNITS == f) convert(there, u, m0 + MS, m0 + 2 * MS, sums);
+                if constexpr (PLAIN) __builtin_amdgcn_sched_barrier(0);
+            }
+            lds_barrier();
+        };
+        for (long long m0 = m_begin; m0 < m_end; m0 += 2 * MS) {             // (a stage behind the end adds nothing)
+            stage(first(), second(), m0);
+            stage(second(), first(), m0 + MS);
         }
-        lds_barrier();
-    }
+    };
+    if (with_bias)                                                          // (shares are never empty)
+        work(std::true_type());
+    else
+        work(std::false_type());
 
+    // the column of G at a place of the tile; a.n where there is none.  A piece that the end cuts holds the last eight columns: the first of them belong to
+    // the piece before it
+    auto output = [&](int at) {
+        const int left = a.n - n0 - (at & ~7);
+        if (!PLAIN || left >= 8 || left <= 0) return n0 + at;
+        const int c = n0 + at - (8 - left);
+        return c >= n0 + (at & ~7) ? c : a.n;
+    };
     // the tile: a lane holds column (lane & 31) and rows 8 (q / 4) + 4 (lane / 32) + q % 4 of each 32 x 32 block
-    auto write = [&](auto one, void* dw, void* db, bool add) {
-        using W = decltype(one);
+    auto write = [&](auto* dw, auto* db) {
+        using W = std::remove_pointer_t<decltype(dw)>;
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -213,32 +251,34 @@ wgrad8_kernel(wgrad8_args a) {
                 const int col = k0 + wk + 32 * j + (lane & 31);
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {
-                    const int row = n0 + wn + 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4;
-                    if (row < a.n && col < a.k) put<W>(dw, (size_t)row * a.k + col, acc[i][j][q], add);
+                    const int row = output(wn + 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4);
+                    if (row < a.n && col < a.k) dw[(size_t)row * a.k + col] = (W)acc[i][j][q];
                 }
             }
         if (with_bias) {                                                    // the same for the whole workgroup
             __syncthreads();
-            float* fold = reinterpret_cast<float*>(&sg[0][0][0]);           // [GROW][TN]
-            static_assert(GROW * TN * 4 <= (int)sizeof(sg), "the column sums fit");
+            float* fold = reinterpret_cast<float*>(&sg0[0][0]);             // [waves][TN]
+            static_assert(WN * WK * TN * 4 <= (int)sizeof(sg0), "the column sums fit");
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fold[grow * TN + gcol + j] = bias[j];
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int off = TN / 8; off < 64; off *= 2) bias[j] += __shfl_xor(bias[j], off);
+                if (lane < TN / 8) fold[wave * TN + gcol + j] = bias[j];
+            }
             __syncthreads();
             for (int c = tid; c < TN; c += THREADS) {
                 float s = 0.f;
-                for (int r = 0; r < GROW; ++r) s += fold[r * TN + c];
-                if (n0 + c < a.n) put<W>(db, n0 + c, s, add);
+                for (int r = 0; r < WN * WK; ++r) s += fold[r * TN + c];
+                if (output(c) < a.n) db[output(c)] = (W)s;
             }
         }
     };
-    if (a.splits > 1)
-        write(float(), (float*)a.dw + (size_t)split * a.n * a.k, (float*)a.db + (size_t)split * a.n, false);
-    else if (a.type == SPF_TYPE_F32)
-        write(float(), a.dw, a.db, a.add != 0);
+    if (a.type == SPF_TYPE_F32)
+        write((float*)a.dw + (size_t)split * a.n * a.k, (float*)a.db + (size_t)split * a.n);
     else if (a.type == SPF_TYPE_BF16)
-        write(__bf16(), a.dw, a.db, a.add != 0);
+        write((__bf16*)a.dw, (__bf16*)a.db);
     else
-        write(_Float16(), a.dw, a.db, a.add != 0);
+        write((_Float16*)a.dw, (_Float16*)a.db);
 }
 
 // out[i] (+)= sum over the splits, in order; eight threads an element group share the splits
@@ -267,21 +307,24 @@ wgrad8_reduce_kernel(const float* __restrict__ tiles, int splits, long long coun
 }
 
 struct plan {
-    int tn, tk, tiles_n, tiles_k, splits;
+    bool big;
+    int tiles_n, tiles_k, splits;
     int64_t share;
 };
 constexpr int STAGE = 32;
+// The loads without conditions need eight columns of G and 32-bit offsets within a stage
+bool plain(int64_t n, int64_t ldg, int type) { return n >= 8 && ldg * type_size(type) < (1ll << 31) / STAGE; }
 // A 256 x 256 tile reads each operand least often and keeps the matrix pipe fed, but a workgroup has a compute unit to itself and leaves 256 KB behind:
 // it is taken where every compute unit gets eight stages of rows or more.  Smaller work takes 64 x 64 tiles, several to a compute unit, and shares as short
 // as two stages, since what counts there is the chain of loads.
 plan plan_of(int64_t rows, int64_t n, int64_t k) {
     plan p;
     const int64_t stages = (rows + STAGE - 1) / STAGE;
-    const bool big = n > 128 && k > 128 && ((n + 255) / 256) * ((k + 255) / 256) * stages >= 256 * 8;
-    p.tn = p.tk = big ? 256 : 64;
-    p.tiles_n = (int)((n + p.tn - 1) / p.tn);
-    p.tiles_k = (int)((k + p.tk - 1) / p.tk);
-    const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, most = big ? 256 : 1024, least = big ? 8 : 2;
+    p.big = n > 128 && k > 128 && ((n + 255) / 256) * ((k + 255) / 256) * stages >= 256 * 8;
+    const int side = p.big ? 256 : 64;
+    p.tiles_n = (int)((n + side - 1) / side);
+    p.tiles_k = (int)((k + side - 1) / side);
+    const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, most = p.big ? 256 : 1024, least = p.big ? 8 : 2;
     int64_t s = most / tiles;
     s = s < stages / least ? s : stages / least;
     s = s < 1 ? 1 : s;
@@ -291,12 +334,14 @@ plan plan_of(int64_t rows, int64_t n, int64_t k) {
     return p;
 }
 
-template <typename T> void launch(const wgrad8_args& a, const plan& p, hipStream_t s) {
+template <typename T> void launch(const wgrad8_args& a, const plan& p, bool is_plain, hipStream_t s) {
     const unsigned wgs = (unsigned)(p.tiles_n * p.tiles_k * p.splits);
-    if (p.tn == 256)
-        wgrad8_kernel<T, 256, 256, 2, 4, STAGE><<<wgs, 512, 0, s>>>(a);
+    if (p.big)
+        wgrad8_kernel<T, 256, 256, 2, 4, STAGE, true><<<wgs, 512, 0, s>>>(a);
+    else if (is_plain)
+        wgrad8_kernel<T, 64, 64, 2, 2, STAGE, true><<<wgs, 256, 0, s>>>(a);
     else
-        wgrad8_kernel<T, 64, 64, 2, 2, STAGE><<<wgs, 256, 0, s>>>(a);
+        wgrad8_kernel<T, 64, 64, 2, 2, STAGE, false><<<wgs, 256, 0, s>>>(a);
 }
 
 const char* bad_sizes(int64_t rows, int64_t n, int64_t k) {
@@ -310,10 +355,10 @@ bool misaligned(const void* p, int size) { return ((uintptr_t)p & (uintptr_t)(si
 
 extern "C" {
 
-int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols) {
+int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t accumulate) {
     if (bad_sizes(rows, n, cols) || rows == 0 || n == 0 || cols == 0) return 0;
     const int64_t splits = plan_of(rows, n, cols).splits;
-    return splits > 1 ? splits * n * (cols + 1) : 0;
+    return splits > 1 || accumulate ? splits * n * (cols + 1) : 0;
 }
 
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols, void* dw, void* db,
@@ -323,18 +368,19 @@ int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, c
     if (const char* why = bad_sizes(rows, n, cols)) return fail(SPF_EINVAL, "%s: %s", who, why);
     if (rows == 0 || n == 0 || cols == 0) return SPF_OK;
     const plan p = plan_of(rows, n, cols);
-    if (!g || !codes || !steps || !dw || (p.splits > 1 && !workspace)) return fail(SPF_EINVAL, "%s: null pointer", who);
-    if (ldg < 0) return fail(SPF_EINVAL, "%s: row stride", who);
+    const bool direct = p.splits == 1 && !accumulate, is_plain = plain(n, ldg, type);
+    if (!g || !codes || !steps || !dw || (!direct && !workspace)) return fail(SPF_EINVAL, "%s: null pointer", who);
+    if (ldg < 0 || (p.big && !is_plain)) return fail(SPF_EINVAL, "%s: a row stride below 0, or of 64 MB or more in a large product", who);
     if (misaligned(g, type_size(type)) || misaligned(codes, 16) || misaligned(dw, type_size(wtype)) || misaligned(db, type_size(wtype)) || misaligned(workspace, 4))
         return fail(SPF_EINVAL, "%s: misaligned pointer", who);
-    float* bias_tiles = db ? workspace + (int64_t)p.splits * n * cols : nullptr;
-    wgrad8_args a = {g, ldg, codes, steps, rows, p.share, (int)n, (int)cols, (int)((cols + S8_BLOCK - 1) / S8_BLOCK), p.tiles_n, p.tiles_k, p.splits, dw, db, wtype, accumulate};
-    if (p.splits > 1) a.dw = workspace, a.db = bias_tiles;
+    wgrad8_args a = {g, ldg, codes, steps, rows, p.share, (int)n, (int)cols, (int)((cols + S8_BLOCK - 1) / S8_BLOCK), p.tiles_n, p.tiles_k, p.splits, dw, db, wtype};
+    float* bias_tiles = db && !direct ? workspace + (int64_t)p.splits * n * cols : nullptr;
+    if (!direct) a.dw = workspace, a.db = bias_tiles, a.type = SPF_TYPE_F32;
     hipStream_t s = (hipStream_t)stream;
-    if (type == SPF_TYPE_F32) launch<float>(a, p, s);
-    else if (type == SPF_TYPE_BF16) launch<__bf16>(a, p, s);
-    else launch<_Float16>(a, p, s);
-    if (p.splits > 1) {
+    if (type == SPF_TYPE_F32) launch<float>(a, p, is_plain, s);
+    else if (type == SPF_TYPE_BF16) launch<__bf16>(a, p, is_plain, s);
+    else launch<_Float16>(a, p, is_plain, s);
+    if (!direct) {
         const int64_t groups = (n * cols + 31) / 32 + (db ? (n + 31) / 32 : 0);
         const auto reduce = [&](auto* w, auto* b) { wgrad8_reduce_kernel<<<(unsigned)groups, 256, 0, s>>>(workspace, p.splits, n * cols, w, bias_tiles, (int)n, b, accumulate); };
         if (wtype == SPF_TYPE_F32) reduce((float*)dw, (float*)db);
