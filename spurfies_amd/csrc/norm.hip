@@ -428,11 +428,17 @@ template <typename T, bool BACKWARD, typename F> void by_width(int cols, F f) {
     }
 #undef SHAPE
 }
-// workgroups that are worth starting: enough waves for the chip, and each with rows enough to pay for its line of column sums
-int groups_of(int64_t rows, int rows_per_group, int threads) {
-    const int64_t most = threads > 256 ? 512 : NORM_GROUPS;
-    const int64_t n = (rows + rows_per_group - 1) / rows_per_group;
-    return (int)(n < most ? n : most);
+// Workgroups for `steps` row steps: as many as the chip holds at once (they walk over the rows), and all with the same number of steps.  More than that run
+// in rounds, the last of which is mostly empty: 1024 of the backward pass at 4096 bf16 columns, of which 768 fit, took 98 us; 745 take 86.
+template <auto KERNEL> int groups_for(int64_t steps, int threads, int64_t most) {
+    static const int resident = [&] {
+        int n = 0;
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) == hipSuccess && n > 0 ? n : 1;
+    }();
+    int64_t slots = 256ll * resident;
+    slots = slots < most ? slots : most;
+    const int64_t rounds = (steps + slots - 1) / slots;
+    return (int)((steps + rounds - 1) / rounds);
 }
 int line_of(int64_t cols) { return (int)((cols + 7) / 8 * 8); }
 
@@ -450,8 +456,8 @@ template <typename T, typename W> void forward(const norm_args& a, hipStream_t s
     }
     by_width<T, false>(a.cols, [&](auto rowt, auto nv) {
         constexpr int ROWT = decltype(rowt)::value, NV = decltype(nv)::value, WG = ROWT < 256 ? 256 : ROWT, RPW = WG / ROWT;
-        const int64_t most = WG > 256 ? 512 : 2048, n = (a.rows + RPW - 1) / RPW;
-        norm_forward_kernel<T, W, ROWT, NV><<<(unsigned)(n < most ? n : most), WG, 0, s>>>(a);
+        const int groups = groups_for<norm_forward_kernel<T, W, ROWT, NV>>((a.rows + RPW - 1) / RPW, WG, 2048);
+        norm_forward_kernel<T, W, ROWT, NV><<<groups, WG, 0, s>>>(a);
     });
 }
 template <typename T, typename W, bool SAVED8> int backward_groups(const norm_args& a, hipStream_t s) {
@@ -466,8 +472,8 @@ template <typename T, typename W, bool SAVED8> int backward_groups(const norm_ar
         return groups;
     }
     by_width<T, true>(a.cols, [&](auto rowt, auto nv) {
-        constexpr int ROWT = decltype(rowt)::value, NV = decltype(nv)::value, WG = ROWT < 256 ? 256 : ROWT;
-        groups = groups_of(a.rows, WG / ROWT, WG);
+        constexpr int ROWT = decltype(rowt)::value, NV = decltype(nv)::value, WG = ROWT < 256 ? 256 : ROWT, RPW = WG / ROWT;
+        groups = groups_for<norm_backward_kernel<T, W, ROWT, NV, SAVED8>>((a.rows + RPW - 1) / RPW, WG, NORM_GROUPS);
         norm_backward_kernel<T, W, ROWT, NV, SAVED8><<<groups, WG, 0, s>>>(a);
     });
     return groups;
