@@ -336,9 +336,12 @@ plan plan_of(int64_t rows, int64_t n, int64_t k) {
 
 template <typename T> void launch(const wgrad8_args& a, const plan& p, bool is_plain, hipStream_t s) {
     const unsigned wgs = (unsigned)(p.tiles_n * p.tiles_k * p.splits);
-    if (p.big)
-        wgrad8_kernel<T, 256, 256, 2, 4, STAGE, true><<<wgs, 512, 0, s>>>(a);
-    else if (is_plain)
+    if (p.big) {
+        // eight waves; the more pieces G has, the fewer of its fragments a wave should read: 64 x 128 outputs a wave take 10 fragments from LDS for 24
+        // products of fp32, 128 x 64 would take 14
+        constexpr int WN = PIECES<T> > 1 ? 4 : 2;
+        wgrad8_kernel<T, 256, 256, WN, 8 / WN, STAGE, true><<<wgs, 512, 0, s>>>(a);
+    } else if (is_plain)
         wgrad8_kernel<T, 64, 64, 2, 2, STAGE, true><<<wgs, 256, 0, s>>>(a);
     else
         wgrad8_kernel<T, 64, 64, 2, 2, STAGE, false><<<wgs, 256, 0, s>>>(a);
