@@ -1962,6 +1962,9 @@ def linear8(x, weight, bias=None, saved=None):
             rows *= k
         if not isinstance(saved, Checkpoint8) or saved.rows != rows or saved.cols != x.shape[-1]:
             raise ValueError("linear8: saved must be the Checkpoint8 of x")
+    if torch.is_autocast_enabled():                            # the product keeps the operands' type, in both passes
+        with torch.autocast("cuda", enabled=False):
+            return linear8(x, weight, bias, saved)
     if not _needs_grad(x, weight, bias):
         return torch.nn.functional.linear(x, weight, bias)
     return _Linear8.apply(x, weight, bias, None if saved is None else saved.codes, None if saved is None else saved.steps)

@@ -115,6 +115,40 @@ def test_offsets_beyond_32_bits():
     assert all(torch.equal(p, q) for p, q in zip(ops.wgrad8(x, ck), ops.wgrad8(small, ck)))
 
 
+def test_more_than_2_31_elements():
+    """70000 x 32768 bf16 in one piece: the last rows come out as they do alone."""
+    from spurfies_amd import ops
+
+    x = torch.full((70000, 32768), 0.5, dtype=torch.bfloat16, device="cuda")
+    tail = randn((3, 32768), torch.bfloat16, 1)
+    x[-3:] = tail
+    ck = ops.checkpoint8(x)
+    small = ops.checkpoint8(tail)
+    assert torch.equal(ck.codes[-3:], small.codes) and torch.equal(ck.steps[-3:], small.steps)
+    assert torch.equal(ck.restore()[-3:], small.restore())
+    del ck
+    assert torch.equal(ops.act8(x, "silu")[-3:], ops.act8(tail, "silu"))
+    assert torch.equal(ops.layer_norm(x)[-3:], ops.layer_norm(tail))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_between_vector_boundaries(dtype):
+    """Views that start at any element, with odd row strides: the same bits as their copies."""
+    from spurfies_amd import ops
+
+    base = randn((40, 1031), dtype, 1)
+    w, b = randn((515,), dtype, 2), randn((515,), dtype, 3)
+    for off in (1, 2, 3, 5):
+        x, g = base[:, off:off + 515], base[:, 515 - off:1030 - off]
+        xs = [x.detach().requires_grad_(True), x.detach().clone().requires_grad_(True)]
+        got = []
+        for v, h in zip(xs, (g, g.clone())):
+            y = ops.layer_norm(v, w, b, saved8=True)
+            z = ops.act8(v, "gelu")
+            got.append((y.detach(), z.detach(), torch.autograd.grad(y, v, h)[0], torch.autograd.grad(z, v, h)[0]) + tuple(ops.wgrad8(h, ops.checkpoint8(v))))
+        assert all(torch.equal(p, q) for p, q in zip(*got)), off
+
+
 # ---- activations ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind,param", KINDS)
@@ -599,6 +633,21 @@ def test_gradients_go_into_their_sinks():
         ops.set_grad_sinks(p.values(), on=False)
     for (k, v), w in zip(p.items(), want):
         assert torch.equal(v.grad, 0.5 + w), k
+
+
+def test_linear8_under_autocast_and_with_frozen_parameters():
+    from spurfies_amd import ops
+
+    x, w, b = randn((60, 96), torch.float32, 1).requires_grad_(True), randn((40, 96), torch.float32, 2).requires_grad_(True), randn((40,), torch.float32, 3).requires_grad_(True)
+    g = randn((60, 40), torch.float32, 4)
+    want = torch.autograd.grad(ops.linear8(x, w, b), (x, w, b), g)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = ops.linear8(x, w, b)
+    assert y.dtype == torch.float32 and all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, w, b), g), want))
+    assert torch.equal(torch.autograd.grad(ops.linear8(x, w.detach(), b.detach()), x, g)[0], want[0])
+    assert torch.equal(torch.autograd.grad(ops.linear8(x.detach(), w, b.detach()), w, g)[0], want[1])
+    assert torch.equal(torch.autograd.grad(ops.linear8(x.detach(), w.detach(), b), b, g)[0], want[2])
+    assert torch.equal(torch.autograd.grad(ops.linear8(x.view(3, 20, 96), w), w, g.view(3, 20, 40))[0], want[1])
 
 
 def test_saved8_keeps_a_quarter_and_forgets_the_input():
