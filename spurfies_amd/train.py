@@ -248,12 +248,14 @@ class TrainStep:
                 # whether and when a rank (re)captures — first step, a new batch shape, parameters re-pointed by load_state_dict — is then
                 # invisible to its peers, whose collective sequences stay aligned (a lone re-capture used to issue
                 # three extra all-reduces and hang the group).
+                # Captured per thread: RCCL's watchdog asks events of earlier eager collectives from its own thread whenever it likes, and a capture
+                # that forbids such calls to every thread ends the process when they meet.
                 pool = torch.cuda.graph_pool_handle()
-                with ops.capture_guard(), torch.cuda.graph(self._graph, pool=pool):
+                with ops.capture_guard(), torch.cuda.graph(self._graph, pool=pool, capture_error_mode="thread_local"):
                     out = self.model(dict(self._static_in, local_data=static_local, iter_step=0), fast=1)
                     self._counts = sdist.fused_counts(out)
                 self._graph_tail = torch.cuda.CUDAGraph()
-                with ops.capture_guard(), torch.cuda.graph(self._graph_tail, pool=pool):
+                with ops.capture_guard(), torch.cuda.graph(self._graph_tail, pool=pool, capture_error_mode="thread_local"):
                     losses = self.loss.fused_forward(out, self._static_gt, denom=self._counts, world=self.world)
                     if not self.zero_in_adam:
                         self.flat.zero_()
