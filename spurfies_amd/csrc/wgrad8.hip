@@ -281,29 +281,34 @@ wgrad8_kernel(wgrad8_args a) {
         write((_Float16*)a.dw, (_Float16*)a.db);
 }
 
-// out[i] (+)= sum over the splits, in order; eight threads an element group share the splits
+// out[i] (+)= sum over the splits: eight threads share them, each takes every eighth in order
 template <typename W>
 __global__ void __launch_bounds__(256)
 wgrad8_reduce_kernel(const float* __restrict__ tiles, int splits, long long count, W* dw, const float* __restrict__ bias_tiles, int n, W* db, int add) {
-    __shared__ float part[8][33];
+    __shared__ float part[8][128];
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const long long groups = (count + 31) / 32;
+    const long long groups = (count + 127) / 128;
     const bool is_bias = blockIdx.x >= groups;                              // the last workgroups add db
-    const long long c = (is_bias ? (long long)blockIdx.x - groups : (long long)blockIdx.x) * 32 + lane;
+    const long long first = (is_bias ? (long long)blockIdx.x - groups : (long long)blockIdx.x) * 128, c = first + 4 * lane;
     const long long len = is_bias ? n : count;
     const float* src = is_bias ? bias_tiles : tiles;
-    float s = 0.f;
-    if (c < len) {
+    float s[4] = {};
 #pragma unroll 8
-        for (int i = k; i < splits; i += 8) s += src[(size_t)i * len + c];
-    }
-    part[k][lane] = s;
-    __syncthreads();
-    if (k != 0 || c >= len) return;
+    for (int i = k; i < splits; i += 8) {
+        const vec_t<float> v = load_vec(src + (size_t)i * len + c, len - c);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][lane];
-    W* out = is_bias ? db : dw;
-    out[c] = (W)(add ? (float)out[c] + s : s);
+        for (int j = 0; j < 4; ++j) s[j] += v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[k][4 * lane + j] = s[j];
+    __syncthreads();
+    const int at = threadIdx.x;
+    if (at >= 128 || first + at >= len) return;
+    float t = part[0][at];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += part[i][at];
+    W* out = (is_bias ? db : dw) + first + at;
+    *out = (W)(add ? (float)*out + t : t);
 }
 
 struct plan {
@@ -384,7 +389,7 @@ int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, c
     else if (type == SPF_TYPE_BF16) launch<__bf16>(a, p, is_plain, s);
     else launch<_Float16>(a, p, is_plain, s);
     if (!direct) {
-        const int64_t groups = (n * cols + 31) / 32 + (db ? (n + 31) / 32 : 0);
+        const int64_t groups = (n * cols + 127) / 128 + (db ? (n + 127) / 128 : 0);
         const auto reduce = [&](auto* w, auto* b) { wgrad8_reduce_kernel<<<(unsigned)groups, 256, 0, s>>>(workspace, p.splits, n * cols, w, bias_tiles, (int)n, b, accumulate); };
         if (wtype == SPF_TYPE_F32) reduce((float*)dw, (float*)db);
         else if (wtype == SPF_TYPE_BF16) reduce((__bf16*)dw, (__bf16*)db);
