@@ -217,7 +217,7 @@ def test_act8_values_that_are_not_finite_and_extremes():
 
 
 # ---- layer norm -------------------------------------------------------------------------------------------------------------------------
-NORM_SHAPES = [(1, 1), (3, 2), (37, 17), (9, 32), (70, 45), (33, 100), (21, 256), (5, 257), (19, 515), (6, 1024), (5, 1500), (4, 2048), (3, 4099), (3, 8192), (2, 9000), (2, 16385)]
+NORM_SHAPES = [(1, 1), (3, 2), (37, 17), (9, 32), (70, 45), (33, 100), (21, 256), (5, 257), (19, 515), (6, 1024), (5, 1500), (4, 2048), (5, 3001), (3, 4099), (3, 8192), (2, 9000), (2, 16385)]
 
 
 def norm_tolerances(X, G, W, B, R, mean, rstd, dtype, wdtype, rows):
@@ -246,7 +246,8 @@ def norm_tolerances(X, G, W, B, R, mean, rstd, dtype, wdtype, rows):
     return y, ty, dx, td, dw, tw, db, tb
 
 
-@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                          (torch.float16, torch.float32)])
 @pytest.mark.parametrize("saved8", [False, True])
 @pytest.mark.parametrize("rows,cols", NORM_SHAPES)
 def test_layer_norm(dtype, wdtype, saved8, rows, cols):
@@ -314,6 +315,32 @@ def test_layer_norm_gradient_against_differences():
             q[i] -= h
             diff[i] = (loss(*[p if j == at else v for j, v in enumerate(args)]) - loss(*[q if j == at else v for j, v in enumerate(args)])) / (2 * h)
         close(got, diff, 2e-5, ("dx", "dw", "db")[at])
+
+
+@pytest.mark.parametrize("make", [lambda x: x[0, 0], lambda x: x, lambda x: x.transpose(0, 2), lambda x: x[:, ::2], lambda x: x[:, :1].expand(4, 7, 40), lambda x: x[:0]])
+def test_shapes_and_strides_of_rows(make):
+    """One dimension, three, a transposed last one, skipped rows, broadcast rows, none: as the dense copy, gradients included."""
+    from spurfies_amd import ops
+
+    x = make(randn((4, 6, 40), torch.float32, 1)).detach()
+    cols = x.shape[-1]
+    w, b = randn((cols,), torch.float32, 2).requires_grad_(True), randn((cols,), torch.float32, 3).requires_grad_(True)
+    m = randn((24, cols), torch.float32, 4).requires_grad_(True)
+    g, h = randn(tuple(x.shape), torch.float32, 5), randn(tuple(x.shape[:-1]) + (24,), torch.float32, 6)
+    got = []
+    for v in (x, x.reshape(-1, cols).clone()):
+        v = v.requires_grad_(True)
+        for saved8 in (False, True):
+            y = ops.layer_norm(v, w, b, saved8=saved8)
+            got.append([y] + list(torch.autograd.grad(y, (v, w, b), g.view(y.shape))))
+        y = ops.act8(v, "gelu")
+        got.append([y] + list(torch.autograd.grad(y, v, g.view(y.shape))))
+        y = ops.linear8(v, m)
+        dx, dm = torch.autograd.grad(y, (v, m), h.view(y.shape))
+        got.append([dm])
+        assert dx.shape == v.shape and y.shape == v.shape[:-1] + (24,)
+    for p, q in zip(got[:4], got[4:]):
+        assert all(torch.equal(i.reshape(j.shape), j) for i, j in zip(p, q))
 
 
 def test_layer_norm_without_parameters_and_partial_gradients():
