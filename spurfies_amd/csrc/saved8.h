@@ -127,18 +127,22 @@ template <int N> __device__ __forceinline__ void s8_mask(uint32_t (&w)[N / 4], l
     }
 }
 __device__ __forceinline__ float s8_step(uint32_t byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23); }
-// the value of byte i of a word
-template <int I> __device__ __forceinline__ float s8_value(uint32_t w, float step) {
-    const float m = (float)((w >> (8 * I)) & 0x7fu) * step;
-    return __uint_as_float(__float_as_uint(m) | ((w << (24 - 8 * I)) & 0x80000000u));
+// The magnitudes of a word's bytes.  The conversions take any byte of a register, if the compiler is kept from folding the mask into a bit-field extract for each.
+__device__ __forceinline__ void s8_magnitudes(uint32_t w, float (&m)[4]) {
+    uint32_t mag = w & 0x7f7f7f7fu;
+    asm("" : "+v"(mag));
+    m[0] = (float)(mag & 0xffu);
+    m[1] = (float)((mag >> 8) & 0xffu);
+    m[2] = (float)((mag >> 16) & 0xffu);
+    m[3] = (float)(mag >> 24);
 }
 template <int N> __device__ __forceinline__ void s8_unpack(const uint32_t (&w)[N / 4], float step, float (&f)[N]) {
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) {
-        f[4 * q] = s8_value<0>(w[q], step);
-        f[4 * q + 1] = s8_value<1>(w[q], step);
-        f[4 * q + 2] = s8_value<2>(w[q], step);
-        f[4 * q + 3] = s8_value<3>(w[q], step);
+        float m[4];
+        s8_magnitudes(w[q], m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * q + i] = __uint_as_float(__float_as_uint(m[i] * step) | ((w[q] << (24 - 8 * i)) & 0x80000000u));
     }
 }
 template <int N> __device__ __forceinline__ void s8_store(uint8_t* codes, size_t at, const uint32_t (&w)[N / 4]) {

@@ -158,11 +158,14 @@ wgrad8_kernel(wgrad8_args a) {
         u32x4 w;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t c = ra[i][2 * h + j], mag = c & 0x7f7f7f7fu;
-            const float v0 = (float)(mag & 0xffu) * step, v1 = (float)((mag >> 8) & 0xffu) * step, v2 = (float)((mag >> 16) & 0xffu) * step, v3 = (float)(mag >> 24) * step;
+            const uint32_t c = ra[i][2 * h + j];
+            float v[4];
+            s8_magnitudes(c, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] *= step;
             // the signs: bytes 0, 1 and 2, 3 moved to the tops of two bf16 pairs
-            w[2 * j] = high_halves(v0, v1) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
-            w[2 * j + 1] = high_halves(v2, v3) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
+            w[2 * j] = high_halves(v[0], v[1]) | (__builtin_amdgcn_perm(0u, c, 0x010c000cu) & 0x80008000u);
+            w[2 * j + 1] = high_halves(v[2], v[3]) | (__builtin_amdgcn_perm(0u, c, 0x030c020cu) & 0x80008000u);
         }
         *reinterpret_cast<u32x4*>(a_of(buf) + (arow + i * AROW) * PK + acol + 8 * h) = w;
     };
