@@ -10,6 +10,8 @@
 // are added through LDS, and one line per workgroup goes to the workspace; a second launch adds the lines in a fixed order.  No atomics: the same
 // call gives the same bits.  Rows too wide for that (forward 16384, backward 8192 columns) are read again for each
 // step — they stay in the caches — with the column sums in a kernel of their own.
+// Measured on MI355X, HBM-bound: 389017 x 256 fp32 147 us forward (5.4 TB/s) and 233 + 6 back (5.1 TB/s); 16384 x 4096 bf16 saved in 8 bits 65 (5.2 TB/s) and
+// 85 + 6 (4.0 TB/s: there the barrier that every row ends in shows, at three workgroups a compute unit).
 #include <math.h>
 
 #include "saved8.h"

@@ -10,6 +10,10 @@
 // row pitch is 64 bytes longer than the tile, so that the four rows of a transposed read lie in different banks.
 // The rows are shared out over enough workgroups to fill the chip.  Each leaves an fp32 tile in the workspace, and a second launch adds them in a
 // fixed order (no atomics: the same call gives the same bits).  db rides along: a loading thread always holds the same eight columns of G.
+//
+// Measured on MI355X: 8192 rows, 4096 x 4096, bf16: 290 us = 948 TFLOP/s (a plain bf16 product of that shape by the library: 280 us); 389017 rows, 256 x 256,
+// fp32: 159 us, of which this kernel 139 (3.6 TB/s of operands; three piece products keep the matrix pipe 49 % busy) and the sum of the splits 12; 1237 rows,
+// 131 x 515, fp16: 9 + 3 us.
 #include "saved8.h"
 
 namespace {
