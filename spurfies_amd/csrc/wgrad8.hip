@@ -4,7 +4,7 @@
 // of two, so that conversion is exact.  G goes to the matrix pipe in bf16 pieces that add up to it exactly — one for bf16, two for fp16, three for fp32
 // (8 bits each, by truncation) — so every product is exact and the only rounding is the fp32 accumulation.
 //
-// A workgroup owns a TN x TK tile of dW over a contiguous share of the rows: a stage of MS rows is loaded to registers while the stage before it is
+// A workgroup owns a TN x TK tile of dW (256, 128 or 64 square) over a contiguous share of the rows: a stage of MS rows is loaded to registers while the stage before it is
 // multiplied, written to LDS row by row (its natural order), and read back transposed: v_mfma_f32_32x32x16_bf16 wants eight consecutive rows of one column
 // in a lane, which is what ds_read_b64_tr_b16 delivers (each group of 16 lanes transposes a 4 x 16 block).  Two LDS buffers, one barrier a stage; the
 // row pitch is 64 bytes longer than the tile, so that the four rows of a transposed read lie in different banks.
@@ -14,6 +14,8 @@
 // Measured on MI355X: 8192 rows, 4096 x 4096, bf16: 290 us = 948 TFLOP/s (a plain bf16 product of that shape by the library: 280 us); 389017 rows, 256 x 256,
 // fp32: 159 us, of which this kernel 139 (3.6 TB/s of operands; three piece products keep the matrix pipe 49 % busy) and the sum of the splits 12; 1237 rows,
 // 131 x 515, fp16: 9 + 3 us.
+#include <math.h>
+
 #include "saved8.h"
 
 namespace {
@@ -318,42 +320,58 @@ wgrad8_reduce_kernel(const float* __restrict__ tiles, int splits, long long coun
     *out = (W)(add ? (float)*out + t : t);
 }
 
-struct plan {
-    bool big;
-    int tiles_n, tiles_k, splits;
-    int64_t share;
-};
 constexpr int STAGE = 32;
 // The loads without conditions need eight columns of G and 32-bit offsets within a stage
 bool plain(int64_t n, int64_t ldg, int type) { return n >= 8 && ldg * type_size(type) < (1ll << 31) / STAGE; }
-// A 256 x 256 tile reads each operand least often and keeps the matrix pipe fed, but a workgroup has a compute unit to itself and leaves 256 KB behind:
-// it is taken where every compute unit gets eight stages of rows or more.  Smaller work takes 64 x 64 tiles, several to a compute unit, and shares as short
-// as two stages, since what counts there is the chain of loads.
-plan plan_of(int64_t rows, int64_t n, int64_t k) {
-    plan p;
+
+struct plan {
+    int side, tiles_n, tiles_k, splits;
+    int64_t share;
+};
+// The tile and the number of row splits with the least estimated time.  A large tile reads its operands least often, but a layer that does not fill it wastes it,
+// and a workgroup with a large tile has a compute unit to itself; splits fill the chip and shorten the chain of stages, but each leaves an fp32 tile that is written
+// and read again.  The constants are microseconds on MI355X: a stage with all its compute unit's workgroups at work, a stage of a workgroup that is alone there,
+// and 5 MB of split tiles.  Measured with the tile set by hand, 256 / 128 / 64 wide: 8192 rows, 4096 x 4096: fp32 641, 797, 1203 us, bf16 288, 369, 601;
+// 389017 rows, 256 x 256, fp32: 162, 219, 358; 400000 rows, 128 x 256, fp32: 157, 109, 169; 1000 rows, 2000 x 2000, bf16: 44, 43, 28.
+struct tile_kind {
+    int side, resident[3];           // workgroups of a compute unit; by SPF_TYPE_*
+    float busy[3], alone[3];
+};
+const tile_kind TILES[] = {{256, {1, 1, 1}, {2.5f, 1.13f, 1.8f}, {1.1f, 1.1f, 1.1f}}, {128, {2, 3, 2}, {1.56f, 1.08f, 1.25f}, {1.0f, 0.75f, 0.85f}},
+                           {64, {3, 5, 4}, {0.88f, 0.73f, 0.8f}, {0.6f, 0.6f, 0.6f}}};
+
+plan plan_of(int64_t rows, int64_t n, int64_t k, int type) {
     const int64_t stages = (rows + STAGE - 1) / STAGE;
-    p.big = n > 128 && k > 128 && ((n + 255) / 256) * ((k + 255) / 256) * stages >= 256 * 8;
-    const int side = p.big ? 256 : 64;
-    p.tiles_n = (int)((n + side - 1) / side);
-    p.tiles_k = (int)((k + side - 1) / side);
-    const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, most = p.big ? 256 : 1024, least = p.big ? 8 : 2;
-    int64_t s = most / tiles;
-    s = s < stages / least ? s : stages / least;
-    s = s < 1 ? 1 : s;
-    const int64_t per = (stages + s - 1) / s;
-    p.splits = (int)((stages + per - 1) / per);
-    p.share = per * STAGE;
-    return p;
+    plan best = {};
+    float least = INFINITY;
+    for (const tile_kind& t : TILES) {
+        if (t.side > 64 && n < 8) continue;                       // (only the 64-wide kernel has a form with conditions)
+        const int64_t tiles_n = (n + t.side - 1) / t.side, tiles_k = (k + t.side - 1) / t.side, tiles = tiles_n * tiles_k, slots = 256 * t.resident[type];
+        for (int64_t want = 1; want <= stages && want <= 1024; want = want < slots / tiles && 2 * want > slots / tiles ? slots / tiles : 2 * want) {
+            const int64_t per = (stages + want - 1) / want, splits = (stages + per - 1) / per, wgs = tiles * splits;
+            const int64_t rounds = (wgs + slots - 1) / slots, beside = wgs >= slots ? t.resident[type] : (wgs + 255) / 256;
+            const float full = t.busy[type] * (float)beside / (float)t.resident[type], stage = full > t.alone[type] ? full : t.alone[type];
+            // (three stages' time to fill and to leave)
+            const float us = (float)rounds * (float)(per + 3) * stage + (splits > 1 ? 3.f + (float)splits * (float)n * (float)k * (8.f / 5e6f) : 0.f);
+            if (us < least) {
+                least = us;
+                best = {t.side, (int)tiles_n, (int)tiles_k, (int)splits, per * STAGE};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T> void launch(const wgrad8_args& a, const plan& p, bool is_plain, hipStream_t s) {
     const unsigned wgs = (unsigned)(p.tiles_n * p.tiles_k * p.splits);
-    if (p.big) {
+    if (p.side == 256) {
         // eight waves; the more pieces G has, the fewer of its fragments a wave should read: 64 x 128 outputs a wave take 10 fragments from LDS for 24
         // products of fp32, 128 x 64 would take 14
         constexpr int WN = PIECES<T> > 1 ? 4 : 2;
         wgrad8_kernel<T, 256, 256, WN, 8 / WN, STAGE, true><<<wgs, 512, 0, s>>>(a);
-    } else if (is_plain)
+    } else if (p.side == 128)
+        wgrad8_kernel<T, 128, 128, 2, 2, STAGE, true><<<wgs, 256, 0, s>>>(a);
+    else if (is_plain)
         wgrad8_kernel<T, 64, 64, 2, 2, STAGE, true><<<wgs, 256, 0, s>>>(a);
     else
         wgrad8_kernel<T, 64, 64, 2, 2, STAGE, false><<<wgs, 256, 0, s>>>(a);
@@ -370,9 +388,9 @@ bool misaligned(const void* p, int size) { return ((uintptr_t)p & (uintptr_t)(si
 
 extern "C" {
 
-int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t accumulate) {
-    if (bad_sizes(rows, n, cols) || rows == 0 || n == 0 || cols == 0) return 0;
-    const int64_t splits = plan_of(rows, n, cols).splits;
+int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t type, int32_t accumulate) {
+    if (bad_sizes(rows, n, cols) || !type_ok(type) || rows == 0 || n == 0 || cols == 0) return 0;
+    const int64_t splits = plan_of(rows, n, cols, type).splits;
     return splits > 1 || accumulate ? splits * n * (cols + 1) : 0;
 }
 
@@ -382,10 +400,10 @@ int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, c
     if (!type_ok(type) || !type_ok(wtype)) return fail(SPF_EINVAL, "%s: unknown element type", who);
     if (const char* why = bad_sizes(rows, n, cols)) return fail(SPF_EINVAL, "%s: %s", who, why);
     if (rows == 0 || n == 0 || cols == 0) return SPF_OK;
-    const plan p = plan_of(rows, n, cols);
+    const plan p = plan_of(rows, n, cols, type);
     const bool direct = p.splits == 1 && !accumulate, is_plain = plain(n, ldg, type);
     if (!g || !codes || !steps || !dw || (!direct && !workspace)) return fail(SPF_EINVAL, "%s: null pointer", who);
-    if (ldg < 0 || (p.big && !is_plain)) return fail(SPF_EINVAL, "%s: a row stride below 0, or of 64 MB or more in a large product", who);
+    if (ldg < 0 || (p.side > 64 && !is_plain)) return fail(SPF_EINVAL, "%s: a row stride below 0, or of 64 MB or more in a large product", who);
     if (misaligned(g, type_size(type)) || misaligned(codes, 16) || misaligned(dw, type_size(wtype)) || misaligned(db, type_size(wtype)) || misaligned(workspace, 4))
         return fail(SPF_EINVAL, "%s: misaligned pointer", who);
     wgrad8_args a = {g, ldg, codes, steps, rows, p.share, (int)n, (int)cols, (int)((cols + S8_BLOCK - 1) / S8_BLOCK), p.tiles_n, p.tiles_k, p.splits, dw, db, wtype};

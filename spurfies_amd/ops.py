@@ -1879,7 +1879,7 @@ def _wgrad8_into(m, ld, codes, steps, cols, dw, db, accumulate):
     rows, n = m.shape
     if ld * m.element_size() >= 1 << 26:                       # rows 64 MB apart: the kernels for large products take 32-bit offsets
         m, ld = m.contiguous(), n
-    ws = torch.empty(_lib.lib().spf_wgrad8_workspace_floats(rows, n, cols, int(accumulate)), dtype=torch.float32, device=m.device)
+    ws = torch.empty(_lib.lib().spf_wgrad8_workspace_floats(rows, n, cols, _TYPES[m.dtype], int(accumulate)), dtype=torch.float32, device=m.device)
     _lib.call("spf_wgrad8", m.device, m.data_ptr(), _TYPES[m.dtype], ld, codes.data_ptr(), steps.data_ptr(), rows, n, cols, dw.data_ptr(), _address(db),
               _TYPES[dw.dtype], int(accumulate), ws.data_ptr())
 

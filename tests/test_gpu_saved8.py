@@ -431,7 +431,8 @@ def test_wgrad8(dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,n,k", [(66001, 256, 130), (66001, 256, 256), (7400, 520, 515), (3300, 1030, 800)])
+@pytest.mark.parametrize("rows,n,k", [(66001, 256, 130), (66001, 256, 256), (7400, 520, 515), (3300, 1030, 800), (100003, 257, 511), (20011, 127, 129), (9000, 1001, 97),
+                                      (2500, 2049, 1030)])
 def test_wgrad8_of_large_layers(dtype, rows, n, k):
     """The wide tiles, with and without split rows and with ragged edges; the restored input is the kernels' own (tested byte for byte above)."""
     from spurfies_amd import ops

@@ -66,7 +66,7 @@ def test_library_refuses_bad_arguments(lib):
     assert back(p, p, p) == -22 and "one of" in err()
     assert back(p, None, None) == -22 and "workspace" in err()
     assert lib.spf_wgrad8(p, 0, 32, p, p, 4, 32, 32, p, None, 5, 0, p, None) == -22 and "type" in err()
-    assert lib.spf_wgrad8_workspace_floats(1 << 16, 32, 32, 0) > 0 and lib.spf_wgrad8_workspace_floats(4, 32, 32, 0) == 0
+    assert lib.spf_wgrad8_workspace_floats(1 << 16, 32, 32, 0, 0) > 0 and lib.spf_wgrad8_workspace_floats(4, 32, 32, 0, 0) == 0
     assert lib.spf_wgrad8(p, 0, 32, p, p, 1 << 16, 32, 32, p, None, 0, 0, None, None) == -22 and "null" in err()
     assert lib.spf_wgrad8(p, 0, 32, q, p, 4, 32, 32, p, None, 0, 0, p, None) == -22 and "misaligned" in err()
     assert lib.spf_wgrad8(p, 0, 32, p, p, 4, 1 << 21, 32, p, None, 0, 0, p, None) == -22 and "2^20" in err()
@@ -77,7 +77,7 @@ def test_nothing_to_do_is_not_an_error(lib):
         assert lib.spf_saved8_pack(None, 0, cols, rows, cols, None, None, None) == 0
         assert lib.spf_saved8_restore(None, None, rows, cols, None, 0, cols, None) == 0
         assert lib.spf_layer_norm_forward(None, 0, cols, rows, cols, None, None, 0, 1e-5, None, cols, None, None, None, None, None, None, None) == 0
-        assert lib.spf_layer_norm_workspace_floats(rows, cols) == 0 and lib.spf_wgrad8_workspace_floats(rows, 8, cols, 1) == 0
+        assert lib.spf_layer_norm_workspace_floats(rows, cols) == 0 and lib.spf_wgrad8_workspace_floats(rows, 8, cols, 0, 1) == 0
         assert lib.spf_wgrad8(None, 0, 8, None, None, rows, 8, cols, None, None, 0, 0, None, None) == 0
 
 
