@@ -1918,7 +1918,9 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, codes, steps):
         y = torch.nn.functional.linear(x, w, b)               # a plain product: the library's
-        if codes is None and any(ctx.needs_input_grad[1:3]):
+        if not any(ctx.needs_input_grad[1:3]):                # frozen parameters: dx needs the weight alone
+            codes = steps = None
+        elif codes is None:
             ck = checkpoint8(x)
             codes, steps = ck.codes, ck.steps
         ctx.save_for_backward(w, codes, steps)
@@ -1955,13 +1957,13 @@ def linear8(x, weight, bias=None, saved=None):
         raise ValueError("linear8: x has no columns")
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise ValueError("linear8: x, weight and bias share one type")
-    _same_device("linear8", x, weight, bias, None if saved is None else saved.codes)
     if saved is not None:
         rows = 1
         for k in x.shape[:-1]:
             rows *= k
         if not isinstance(saved, Checkpoint8) or saved.rows != rows or saved.cols != x.shape[-1]:
             raise ValueError("linear8: saved must be the Checkpoint8 of x")
+    _same_device("linear8", x, weight, bias, None if saved is None else saved.codes)
     if torch.is_autocast_enabled():                            # the product keeps the operands' type, in both passes
         with torch.autocast("cuda", enabled=False):
             return linear8(x, weight, bias, saved)

@@ -738,6 +738,10 @@ def test_gpu_refusals():
         ops.linear8(x, torch.zeros(8, 32, device="cuda", dtype=torch.float16))
     with pytest.raises(ValueError, match="Checkpoint8 of x"):
         ops.linear8(x, torch.zeros(8, 32, device="cuda"), saved=ops.checkpoint8(torch.zeros(5, 32, device="cuda")))
+    with pytest.raises(ValueError, match="Checkpoint8 of x"):
+        ops.linear8(x, torch.zeros(8, 32, device="cuda"), saved=x)
+    with pytest.raises(ValueError, match="devices"):
+        ops.linear8(x, torch.zeros(8, 32))
     x.requires_grad_(True)
     w = torch.zeros(8, 32, device="cuda")
     for y in (ops.act8(x, "silu"), ops.layer_norm(x), ops.linear8(x, w)):
