@@ -81,7 +81,7 @@ act8_forward_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ y, l
         row[u] = m.per_row(b);
         col[u] = (long long)(b - row[u] * m.per_row.d) * S8_BLOCK + c;
         left[u] = b < m.n_blocks ? m.cols - col[u] : 0;
-        raw[u] = load_vec(x + (long long)row[u] * ldx + col[u], left[u]);
+        raw[u] = load_vec(x + (long long)row[u] * ldx + col[u], left[u], col[u] > 0);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -133,7 +133,7 @@ act8_backward_kernel(const T* __restrict__ dy, long long ldy, const uint8_t* __r
         if (left[u] > 0) {
             s8_load<V>(codes, (size_t)b * S8_BLOCK + c, w[u]);
             e[u] = steps[b];
-            if (KIND != KIND_NONE) raw[u] = load_vec(dy + (long long)row[u] * ldy + col[u], left[u]);
+            if (KIND != KIND_NONE) raw[u] = load_vec(dy + (long long)row[u] * ldy + col[u], left[u], col[u] > 0);
         }
     }
 #pragma unroll

@@ -90,7 +90,7 @@ norm_forward_kernel(norm_args a) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * ROWT + t) * V;
-            next[v] = load_vec(x + row * a.ldx + c, row < a.rows ? a.cols - c : 0);
+            next[v] = load_vec(x + row * a.ldx + c, row < a.rows ? a.cols - c : 0, c > 0);
         }
     };
     const float inv_cols = 1.f / (float)a.cols;
@@ -175,7 +175,7 @@ norm_backward_kernel(norm_args a) {
         for (int v = 0; v < NV; ++v) {
             const int c = (v * ROWT + t) * V;
             const long long n = ok ? a.cols - c : 0;
-            next_g[v] = load_vec((const T*)a.dy + row * a.ldd + c, n);
+            next_g[v] = load_vec((const T*)a.dy + row * a.ldd + c, n, c > 0);
             if constexpr (SAVED8) {
                 next_e[v] = 0;
 #pragma unroll
@@ -185,7 +185,7 @@ norm_backward_kernel(norm_args a) {
                     next_e[v] = a.in_steps[(size_t)row * nb + c / S8_BLOCK];
                 }
             } else {
-                next_x[v] = load_vec((const T*)a.x + row * a.ldx + c, n);
+                next_x[v] = load_vec((const T*)a.x + row * a.ldx + c, n, c > 0);
             }
         }
         next_mean = ok ? a.mean[row] : 0.f;
@@ -274,14 +274,14 @@ norm_wide_forward_kernel(norm_args a) {
     const float inv_cols = 1.f / (float)a.cols;
     float f[V], s = 0.f;
     for (long long c = threadIdx.x * V; c < a.cols; c += STEP) {
-        to_f32<T>(load_vec(x + c, a.cols - c), f);
+        to_f32<T>(load_vec(x + c, a.cols - c, c > 0), f);
 #pragma unroll
         for (int i = 0; i < V; ++i) s += f[i];
     }
     const float mean = row_sum<1024>(s, red[0]) * inv_cols;
     float q = 0.f;
     for (long long c = threadIdx.x * V; c < a.cols; c += STEP) {
-        to_f32<T>(load_vec(x + c, a.cols - c), f);
+        to_f32<T>(load_vec(x + c, a.cols - c, c > 0), f);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float d = c + i < a.cols ? f[i] - mean : 0.f;
@@ -293,7 +293,7 @@ norm_wide_forward_kernel(norm_args a) {
     for (long long at = 0; at < a.cols; at += STEP) {                   // whole waves (a block's lanes work together)
         const long long c = at + threadIdx.x * V, left = a.cols - c;
         uint32_t k[V / 4];
-        to_f32<T>(load_vec(x + c, left), f);
+        to_f32<T>(load_vec(x + c, left, c > 0), f);
         if (a.in_codes) {
             const uint32_t e = s8_pack(f, k);
             s8_mask<V>(k, left);
@@ -329,7 +329,7 @@ template <typename T, bool SAVED8> __device__ __forceinline__ void normalised(co
         s8_load<V>(a.in_codes, (size_t)row * nb * S8_BLOCK + c, k);
         s8_unpack<V>(k, s8_step(a.in_steps[(size_t)row * nb + c / S8_BLOCK]), n);
     } else {
-        to_f32<T>(load_vec((const T*)a.x + row * a.ldx + c, a.cols - c), n);
+        to_f32<T>(load_vec((const T*)a.x + row * a.ldx + c, a.cols - c, c > 0), n);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) n[i] = c + i < a.cols ? (n[i] - mean) * rstd : 0.f;
@@ -347,7 +347,7 @@ norm_wide_backward_kernel(norm_args a) {
     const float mean = a.mean[row], rstd = a.rstd[row], inv_cols = 1.f / (float)a.cols;
     float n[V], g[V], w[V], c1 = 0.f, c2 = 0.f;
     for (long long c = threadIdx.x * V; c < a.cols; c += STEP) {
-        to_f32<T>(load_vec(dy + c, a.cols - c), g);
+        to_f32<T>(load_vec(dy + c, a.cols - c, c > 0), g);
         normalised<T, SAVED8>(a, row, c, nb, mean, rstd, n);
         load_weights<W>(a.w, c, a.cols, 1.f, w);
 #pragma unroll
@@ -360,7 +360,7 @@ norm_wide_backward_kernel(norm_args a) {
     row_sum2<1024>(c1, c2, red);
     c1 *= inv_cols, c2 *= inv_cols;
     for (long long c = threadIdx.x * V; c < a.cols; c += STEP) {
-        to_f32<T>(load_vec(dy + c, a.cols - c), g);
+        to_f32<T>(load_vec(dy + c, a.cols - c, c > 0), g);
         normalised<T, SAVED8>(a, row, c, nb, mean, rstd, n);
         load_weights<W>(a.w, c, a.cols, 1.f, w);
 #pragma unroll
@@ -381,7 +381,7 @@ norm_wide_columns_kernel(norm_args a) {
     if (c >= a.cols) return;
     float dw[V] = {}, db[V] = {}, n[V], g[V];
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        to_f32<T>(load_vec((const T*)a.dy + row * a.ldd + c, a.cols - c), g);
+        to_f32<T>(load_vec((const T*)a.dy + row * a.ldd + c, a.cols - c, c > 0), g);
         normalised<T, SAVED8>(a, row, c, nb, a.mean[row], a.rstd[row], n);
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[i] += g[i] * n[i], db[i] += g[i];

@@ -101,7 +101,7 @@ wgrad8_kernel(wgrad8_args a) {
             const uint32_t at = min((uint32_t)(grow + i * GROW), (uint32_t)(m_end - 1 - m)) * (uint32_t)g_row + (uint32_t)g_at * (uint32_t)sizeof(T);
             const T* p = reinterpret_cast<const T*>((const uint8_t*)a.g + m * g_row + at);
 #pragma unroll
-            for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = *reinterpret_cast<const vec_any_t<T>*>(p + q * VEC<T>);
+            for (int q = 0; q < 8 / VEC<T>; ++q) rg[i][q] = load_any(p + q * VEC<T>);
         } else {
             const long long m = m0 + grow + i * GROW;
             const int left = m < m_end ? g_left : 0;
