@@ -25,14 +25,43 @@ struct rows8 {                               // the blocks of a matrix, numbered
     long long cols;
 };
 
-// e^x: the hardware's 2^x of a rounded product, so the result carries |x| / 2^24 more relative error than a correctly rounded one — of a value that is e^x,
-// which leaves less than 2^-24 of the sums it enters here
-__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+// What follows comes in two forms.  FINE, for fp32: errors of a few units of 2^-24 relative to the result, wherever that lies (such passes are bound by HBM with room
+// for it).  The other, for 16-bit results: short, with relative errors of 2^-16 and less where half a step of the result is 2^-12 or more.
 
+// e^-(x + lo) for x >= 0 and a small lo.  The hardware's 2^t takes a rounded t = -x log2 e, off by up to x / 2^24; FINE puts that back: e^-x = 2^t (1 + r ln 2) with
+// t + r = -x log2 e.  Beyond x = 200 all of it is zero (the bound keeps infinities out of r).
+template <bool FINE> __device__ __forceinline__ float exp_neg(float x, float lo) {
+    constexpr float L = 1.44269504088896341f, L_LOW = 1.92596299e-8f, LN2 = 0.693147180559945309f;         // log2 e = L + L_LOW
+    if (!FINE) return __builtin_amdgcn_exp2f(x * -L);
+    lo = x < 200.f ? lo : 0.f;
+    x = fminf(x, 200.f);
+    const float t = x * -L;
+    float r = __builtin_fmaf(x, -L, -t);
+    r = __builtin_fmaf(x, -L_LOW, r);
+    r = __builtin_fmaf(lo, -L, r);
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e * LN2, r, e);
+}
+// 1 / d; FINE: with a step of Newton's
+template <bool FINE> __device__ __forceinline__ float inverse(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return FINE ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r) : r;
+}
+// 1 / (1 + e^-v), and 1 minus that.  FINE: from e^-|v|, which neither overflows nor cancels; lo: v's rounding.  (In 16 bits that form costs 3 - 4 % of SiLU's passes.)
+template <bool FINE> __device__ __forceinline__ float sigmoid(float v, float lo, float& other) {
+    if (!FINE) {
+        const float s = inverse<false>(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
+        other = 1.f - s;
+        return s;
+    }
+    const float a = exp_neg<true>(fabsf(v), v > 0.f ? lo : -lo), r = inverse<true>(1.f + a), q = a * r;
+    other = v > 0.f ? q : r;
+    return v > 0.f ? r : q;
+}
 // The normal distribution's P(Z > |v|) by Hastings' approximation (Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erfc within 1.5e-7), and
 // e^(-v^2 / 2) beside it, which both GELU and its derivative need: a third of the instructions of erf and exp
 __device__ __forceinline__ float normal_tail(float v, float& bell) {
-    bell = exp_fast(-0.5f * v * v);
+    bell = exp_neg<false>(0.5f * v * v, 0.f);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(v), 0.3275911f * 0.70710678118654752f, 1.f));
     float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
     p = __builtin_fmaf(t, p, 1.421413741f);
@@ -41,24 +70,31 @@ __device__ __forceinline__ float normal_tail(float v, float& bell) {
     return 0.5f * t * p * bell;
 }
 
-template <int KIND> __device__ __forceinline__ float act(float v, float p, float ip) {
+template <int KIND, bool FINE> __device__ __forceinline__ float act(float v, float p, float ip) {
     if (KIND == SPF_ACT_LEAKY_RELU) return v > 0.f ? v : v * p;
     if (KIND == SPF_ACT_SOFTPLUS) {
-        const float z = v * p;
-        return v != v ? v : (fmaxf(z, 0.f) + log1pf(exp_fast(-fabsf(z)))) * ip;   // (fmaxf drops a NaN)
+        const float z = v * p, lo = __builtin_fmaf(v, p, -z);
+        return v != v ? v : (fmaxf(z, 0.f) + log1pf(exp_neg<FINE>(fabsf(z), z > 0.f ? lo : -lo))) * ip;   // (fmaxf drops a NaN)
     }
-    if (KIND == SPF_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + exp_fast(-v));
+    if (KIND == SPF_ACT_SILU) {
+        float other;
+        return v * sigmoid<FINE>(v, 0.f, other);
+    }
     float bell;
     const float tail = normal_tail(v, bell);
     return v * (v > 0.f ? 1.f - tail : tail);
 }
 // f'(v); LeakyReLU: from the sign of the restored value, which is the sign of the element (a restored NaN stays one)
-template <int KIND> __device__ __forceinline__ float act_slope(float v, float p) {
+template <int KIND, bool FINE> __device__ __forceinline__ float act_slope(float v, float p) {
     if (KIND == SPF_ACT_LEAKY_RELU) return v != v ? v : ((int)__float_as_uint(v) < 0 ? p : 1.f);
-    if (KIND == SPF_ACT_SOFTPLUS) return __builtin_amdgcn_rcpf(1.f + exp_fast(-v * p));
+    float other;
+    if (KIND == SPF_ACT_SOFTPLUS) {
+        const float z = v * p, s = sigmoid<FINE>(z, __builtin_fmaf(v, p, -z), other);
+        return v != v ? v : s;
+    }
     if (KIND == SPF_ACT_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.f + exp_fast(-v));
-        return s * (1.f + v * (1.f - s));
+        const float s = sigmoid<FINE>(v, 0.f, other);
+        return s * (1.f + v * other);
     }
     float bell;
     const float tail = normal_tail(v, bell);
@@ -98,7 +134,7 @@ act8_forward_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ y, l
         }
         if (KIND != KIND_NONE) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = act<KIND>(f[i], p, ip);
+            for (int i = 0; i < V; ++i) f[i] = act<KIND, sizeof(T) == 4>(f[i], p, ip);
             const vec_t<T> out = from_f32<T>(f);
             store_vec(y + (long long)row[u] * ldy + col[u], out, left[u]);
             if (out_codes) {                                       // the bytes of y as the next layer sees it
@@ -144,7 +180,7 @@ act8_backward_kernel(const T* __restrict__ dy, long long ldy, const uint8_t* __r
         if (KIND != KIND_NONE) {
             to_f32<T>(raw[u], g);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = g[i] * act_slope<KIND>(f[i], p);
+            for (int i = 0; i < V; ++i) f[i] = g[i] * act_slope<KIND, sizeof(T) == 4>(f[i], p);
         } else if (sizeof(T) == 2 && (float)(T)65504.f == 65504.f) {
             // fp16's largest numbers round up to 65536: the largest finite one stands for them (and for anything larger from a wider type)
 #pragma unroll

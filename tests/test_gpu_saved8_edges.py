@@ -1,0 +1,76 @@
+"""The training operators with 8-bit saved activations at the edges of what their documentation allows: far arguments, values that are not finite, autocast,
+shared parameters, sizes beyond a launch's limits, and shapes that reach every form of the kernels.  Tolerances count roundings: u = 2^-24, half(type) = finfo.eps / 2."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import saved8 as O
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """the spacing of the type's smallest numbers"""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def randn(shape, dtype, seed, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype).cuda()
+
+
+def close(got, want, tol, what):
+    got = f64(got) if torch.is_tensor(got) else got
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.size} off, worst {np.nanmax(np.abs(got - want) / np.maximum(tol, 1e-300)):.3g} times the tolerance"
+
+
+# ---- activations far from zero ----------------------------------------------------------------------------------------------------------
+def passes(x, kind, param):
+    """y, dx for a gradient of ones, and the 64-bit values of x and of its restored 8-bit form"""
+    from spurfies_amd import ops
+
+    x = x.requires_grad_(True)
+    y = ops.act8(x, kind, param=param)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    return y, dx, f64(x), O.restore(*O.pack(f64(x)), x.shape[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu_is_exact_to_its_last_digits_wherever_it_lies(dtype):
+    """Relative to the result.  e^-|x| has the hardware's 2 u and up to 5 u around it; 1 + it, its inverse and three products another 7 (fp32: K = 14); 16-bit results
+    take the exponential of a rounded product, 1.3 |x| u more.  The hardware's 2^t has nothing below the smallest normal number: 2^-126 of it, times x."""
+    x = torch.linspace(-100.0, 20.0, 64 * 96).view(64, 96).to(dtype).cuda()
+    y, dx, X, R = passes(x, "silu", None)
+    k = lambda z: 14 + (0 if dtype == torch.float32 else 2 * np.abs(z))  # noqa: E731
+    with np.errstate(over="ignore"):
+        s, o = 1 / (1 + np.exp(-X)), 1 / (1 + np.exp(X))
+        close(y, X * s, (half(dtype) + k(X) * U) * np.abs(X * s) + np.abs(X) * 2.0 ** -126 + tiny(dtype), "y")
+        s, o = 1 / (1 + np.exp(-R)), 1 / (1 + np.exp(R))
+    # the slope's two terms, s and s x (1 - s)
+    close(dx, s * (1 + R * o), half(dtype) * np.abs(s * (1 + R * o)) + 2 * k(R) * U * s * (1 + np.abs(R) * o) + (1 + np.abs(R)) * 2.0 ** -126 + tiny(dtype), "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softplus_is_exact_to_its_last_digits_wherever_it_lies(dtype):
+    """As SiLU, with z = beta x: its rounding counts |z| u unless it is carried along (fp32); the logarithm adds 4 u, 1 / beta and the sum 3."""
+    beta = 100.0
+    x = torch.linspace(-0.85, 0.3, 64 * 96).view(64, 96).to(dtype).cuda()
+    y, dx, X, R = passes(x, "softplus", beta)
+    k = lambda z: 21 + (0 if dtype == torch.float32 else 3 * np.abs(z))  # noqa: E731
+    want = np.logaddexp(0.0, beta * X) / beta
+    close(y, want, (half(dtype) + k(beta * X) * U) * want + 2.0 ** -126 + tiny(dtype), "y")
+    want = 1 / (1 + np.exp(-beta * R))
+    close(dx, want, (half(dtype) + k(beta * R) * U) * want + 2.0 ** -126 + tiny(dtype), "dx")
