@@ -72,9 +72,9 @@ __device__ __forceinline__ float normal_tail(float v, float& bell) {
 
 template <int KIND, bool FINE> __device__ __forceinline__ float act(float v, float p, float ip) {
     if (KIND == SPF_ACT_LEAKY_RELU) return v > 0.f ? v : v * p;
-    if (KIND == SPF_ACT_SOFTPLUS) {
+    if (KIND == SPF_ACT_SOFTPLUS) {                                                // log(1 + e^z) / p = max(v, 0) + log(1 + e^-|z|) / p, z = p v
         const float z = v * p, lo = __builtin_fmaf(v, p, -z);
-        return v != v ? v : (fmaxf(z, 0.f) + log1pf(exp_neg<FINE>(fabsf(z), z > 0.f ? lo : -lo))) * ip;   // (fmaxf drops a NaN)
+        return v != v ? v : fmaxf(v, 0.f) + log1pf(exp_neg<FINE>(fabsf(z), z > 0.f ? lo : -lo)) * ip;     // (fmaxf drops a NaN)
     }
     if (KIND == SPF_ACT_SILU) {
         float other;

@@ -74,3 +74,14 @@ def test_softplus_is_exact_to_its_last_digits_wherever_it_lies(dtype):
     close(y, want, (half(dtype) + k(beta * X) * U) * want + 2.0 ** -126 + tiny(dtype), "y")
     want = 1 / (1 + np.exp(-beta * R))
     close(dx, want, (half(dtype) + k(beta * R) * U) * want + 2.0 ** -126 + tiny(dtype), "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softplus_of_values_whose_product_with_beta_overflows(dtype):
+    """beta x beyond fp32's range: y is x, and nothing on the other side."""
+    from spurfies_amd import ops
+
+    big = float(torch.finfo(dtype).max)
+    x = torch.tensor([[big, -big, big / 2, 1.0] * 8]).to(dtype).cuda()
+    y = ops.act8(x, "softplus", param=1e38)
+    assert torch.equal(y, x.clamp(min=0))
