@@ -85,3 +85,30 @@ def test_softplus_of_values_whose_product_with_beta_overflows(dtype):
     x = torch.tensor([[big, -big, big / 2, 1.0] * 8]).to(dtype).cuda()
     y = ops.act8(x, "softplus", param=1e38)
     assert torch.equal(y, x.clamp(min=0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu_is_exact_to_its_last_digits_wherever_it_lies(dtype):
+    """Relative to the result, also in the far negative tail.  fp32: the approximation of the tail is off by 0.4 u, the exponential beside it by 7, eight steps of the
+    polynomial, an inverse and three products by another 12 (K = 20).  16-bit results: an approximation within 15 u, an exponential off by x^2 / 2 * 1.3 u."""
+    x = torch.linspace(-12.5, 6.0, 64 * 96).view(64, 96).to(dtype).cuda()
+    y, dx, X, R = passes(x, "gelu", None)
+    from scipy.special import erfc
+
+    k = lambda z: 20 + (0 if dtype == torch.float32 else 15 + z * z)  # noqa: E731
+    cdf = lambda z: 0.5 * erfc(-z / np.sqrt(2))  # noqa: E731
+    close(y, X * cdf(X), (half(dtype) + k(X) * U) * np.abs(X * cdf(X)) + np.abs(X) * 2.0 ** -126 + tiny(dtype), "y")
+    bell = R * np.exp(-R * R / 2) / np.sqrt(2 * np.pi)
+    close(dx, cdf(R) + bell, half(dtype) * np.abs(cdf(R) + bell) + k(R) * U * (cdf(R) + np.abs(bell)) + (1 + np.abs(R)) * 2.0 ** -126 + tiny(dtype), "dx")
+
+
+def test_gelu_in_32_bits_is_as_exact_as_its_formula():
+    """Near zero, where the inputs are: 0.5 x (1 + erf(x / sqrt 2)) in fp32 has the roundings of the product, erf (2 u), the sum and two more; a cdf of a half to within
+    1.5 u of one, i.e. 3 u of the result, and one for the last product."""
+    x = randn((512, 256), torch.float32, 5, scale=0.3)
+    y, _, X, _ = passes(x, "gelu", None)
+    from scipy.special import erfc
+
+    want = X * 0.5 * erfc(-X / np.sqrt(2))
+    assert np.linalg.norm(f64(y) - want) < 1.0 * U * np.linalg.norm(want)          # (independent roundings: their root mean square)
+    close(y, want, 5 * U * np.abs(want) + tiny(torch.float32), "y")
