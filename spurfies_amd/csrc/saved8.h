@@ -119,10 +119,9 @@ template <int N> __device__ __forceinline__ uint32_t s8_pack(const float (&f)[N]
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float v = f[4 * q + i];
-            const uint32_t b = __float_as_uint(v);
             // 2^23 + |v| / 2^s rounds to a whole number, ties to even, in the low bits (the product is exact)
             m[i] = __float_as_uint(fminf(__builtin_fmaf(fabsf(v), inv, 8388608.0f), 8388608.0f + 127.0f));
-            n[i] = b | (b - 1u);                                                              // top bit: not greater than zero
+            n[i] = v > 0.f ? 0u : 0x80000000u;                                                // top bit: not greater than zero (as a NaN is not)
         }
         const uint32_t mag = __builtin_amdgcn_perm(__builtin_amdgcn_perm(m[3], m[2], 0x0c0c0400u), __builtin_amdgcn_perm(m[1], m[0], 0x0c0c0400u), 0x05040100u);
         const uint32_t sgn = __builtin_amdgcn_perm(__builtin_amdgcn_perm(n[3], n[2], 0x0c0c0703u), __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0703u), 0x05040100u);

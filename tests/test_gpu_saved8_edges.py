@@ -112,3 +112,20 @@ def test_gelu_in_32_bits_is_as_exact_as_its_formula():
     want = X * 0.5 * erfc(-X / np.sqrt(2))
     assert np.linalg.norm(f64(y) - want) < 1.0 * U * np.linalg.norm(want)          # (independent roundings: their root mean square)
     close(y, want, 5 * U * np.abs(want) + tiny(torch.float32), "y")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_bytes_of_blocks_that_are_not_finite(dtype):
+    """The sign bit says "not greater than zero" there as well: a NaN, of either sign, is not."""
+    from spurfies_amd import ops
+
+    nan, inf = float("nan"), float("inf")
+    x = torch.tensor([[nan, 1.0, -1.0, 0.0] * 16, [inf, -inf, 2.0, -2.0] * 16, [1.0] * 40 + [nan] * 24]).to(dtype).cuda()
+    x[2, 50:] = -x[2, 50:]
+    ck = ops.checkpoint8(x)
+    codes, steps = O.pack(f64(x))
+    assert np.array_equal(ck.steps.cpu().numpy(), steps) and np.array_equal(ck.codes.cpu().numpy(), codes)
+    # LayerNorm's and the activations' 8-bit forms are written by the same code
+    for form in (ops.layer_norm(x, out8=True), ops.act8(x, "leaky_relu", out8=True)):
+        assert torch.equal(form[1].codes, ops.checkpoint8(form[0]).codes)
+        assert np.array_equal(form[1].codes.cpu().numpy(), O.pack(f64(form[0]))[0])
