@@ -1914,6 +1914,14 @@ def wgrad8(g, saved, out=None, dbias=None, bias=True):
     return dw, db
 
 
+def _product(a, b):
+    """a @ b in the operands' type (the engine runs backward passes under the autocast state of whoever asked for them)."""
+    if not torch.is_autocast_enabled(a.device.type):
+        return a @ b
+    with torch.autocast(a.device.type, enabled=False):
+        return a @ b
+
+
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, codes, steps):
@@ -1934,7 +1942,7 @@ class _Linear8(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         m, ld = _rows_of(g, "linear8")
         n, cols = w.shape
-        dx = (m @ w).view(g.shape[:-1] + (cols,)) if need_x else None
+        dx = _product(m, w).view(g.shape[:-1] + (cols,)) if need_x else None
         if not need_w and not need_b:
             return dx, None, None, None, None
         if ctx.sinks is not None:

@@ -129,3 +129,17 @@ def test_bytes_of_blocks_that_are_not_finite(dtype):
     for form in (ops.layer_norm(x, out8=True), ops.act8(x, "leaky_relu", out8=True)):
         assert torch.equal(form[1].codes, ops.checkpoint8(form[0]).codes)
         assert np.array_equal(form[1].codes.cpu().numpy(), O.pack(f64(form[0]))[0])
+
+
+# ---- linear8 ----------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear8_keeps_its_type_where_the_backward_pass_runs_under_autocast(dtype):
+    from spurfies_amd import ops
+
+    x, w, b = randn((60, 96), dtype, 1).requires_grad_(True), randn((40, 96), dtype, 2).requires_grad_(True), randn((40,), dtype, 3).requires_grad_(True)
+    g = randn((60, 40), dtype, 4)
+    want = torch.autograd.grad(ops.linear8(x, w, b), (x, w, b), g)
+    for other in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", dtype=other):
+            got = torch.autograd.grad(ops.linear8(x, w, b), (x, w, b), g)
+        assert all(p.dtype == dtype and torch.equal(p, q) for p, q in zip(got, want))
