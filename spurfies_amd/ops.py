@@ -6,6 +6,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _prof
 
@@ -1692,6 +1693,14 @@ def _bytes8(rows, cols):
     return rows * blocks * 32, rows * blocks * 33
 
 
+def _no_tangents(who, *tensors):
+    """Refuse forward-mode derivatives: a dual tensor has a data pointer and needs no gradient, so its tangent would be dropped in silence."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who}: there is no forward-mode derivative")
+
+
 def _needs_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -1761,6 +1770,7 @@ def act8(x, kind, param=None, out8=False):
         raise ValueError("act8: softplus needs beta > 0")
     if x.dim() == 0:
         raise ValueError("act8: needs at least one dimension")
+    _no_tangents("act8", x)
     if _needs_grad(x):
         r = _Act8.apply(x, number, param, bool(out8))
         if not out8:
@@ -1863,6 +1873,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError("layer_norm: eps must be finite and not negative")
+    _no_tangents("layer_norm", x, *params)
     if _needs_grad(x, weight, bias):
         r = _LayerNorm.apply(x, weight, bias, eps, bool(saved8), bool(out8))
         if not out8:
@@ -1886,7 +1897,7 @@ def _wgrad8_into(m, ld, codes, steps, cols, dw, db, accumulate):
 
 def wgrad8(g, saved, out=None, dbias=None, bias=True):
     """(dW [n, cols], db [n]) of a linear layer from the gradient g [..., n] of its output and its saved input (spf_wgrad8): dW = g^T a, db = column sums.
-    New fp32 tensors — bias=False: db is None — or, with out (and dbias), += into those (one type, any of the three; contiguous)."""
+    New fp32 tensors — bias=False: db is None — or, with out (and dbias), += into those (one type, any of the three; contiguous).  No gradient flows through it."""
     _type_of(g, "wgrad8")
     if not isinstance(saved, Checkpoint8):
         raise ValueError("wgrad8: saved must be a Checkpoint8")

@@ -16,6 +16,28 @@ def no_kernels(monkeypatch):
     return calls
 
 
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(no_kernels, grad):
+    """A dual tensor needs no gradient and has a data pointer: without a refusal its tangent would be dropped."""
+    x, w, b = torch.randn(4, 32), torch.randn(32), torch.randn(32)
+    with fwAD.dual_level(), torch.set_grad_enabled(grad):
+        d, dw = fwAD.make_dual(x, torch.ones_like(x)), fwAD.make_dual(w, torch.ones_like(w))
+        for call in (lambda: ops.act8(d, "silu"), lambda: ops.act8(d, "gelu", out8=True), lambda: ops.layer_norm(d, w, b), lambda: ops.layer_norm(x, dw, b),
+                     lambda: ops.layer_norm(x, w, dw, saved8=True)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert not no_kernels
+        ops.layer_norm(x, w, b)                                              # plain tensors pass
+        ops.act8(x, "silu")
+        assert len(no_kernels) == 2
+        # linear8 without a graph is the library's product, which has the derivative
+        m = torch.randn(8, 32)
+        assert torch.equal(fwAD.unpack_dual(ops.linear8(d, m)).tangent, torch.ones_like(x) @ m.t())
+        if grad:
+            with pytest.raises(RuntimeError):
+                ops.linear8(d, m.requires_grad_(True))
+
+
 def test_linear8_backward_keeps_its_type_under_autocast():
     """The engine carries the caller's autocast state into the backward pass (here the CPU's, with frozen parameters: no kernel is reached)."""
     x, w, g = torch.randn(5, 64, requires_grad=True), torch.randn(8, 64), torch.randn(5, 8)
