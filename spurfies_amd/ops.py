@@ -1732,6 +1732,7 @@ def _act8_forward(x, kind, param, train, out8):
 class _Act8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kind, param, out8):
+        ctx.set_materialize_grads(False)                      # codes and steps have no gradient: no zeros of their size either
         y, kept, codes, steps = _act8_forward(x, kind, param, True, out8)
         ctx.save_for_backward(*((codes, steps) if kept is None else (kept,)))
         ctx.kind, ctx.param = kind, param
@@ -1742,6 +1743,8 @@ class _Act8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, *_):
+        if g is None:
+            return None, None, None, None
         _once("act8")
         saved = ctx.saved_tensors
         m, ld = _rows_of(g, "act8")
@@ -1817,6 +1820,7 @@ def _layer_norm_forward(x, w, b, eps, train, saved8, out8):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, eps, saved8, out8):
+        ctx.set_materialize_grads(False)
         y, used, stat, kept, codes, steps = _layer_norm_forward(x, w, b, eps, True, saved8, out8)
         ctx.save_for_backward(None if saved8 else used, stat, kept, w)
         ctx.wdtype = (x if w is None and b is None else b if w is None else w).dtype
@@ -1828,6 +1832,8 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, *_):
+        if g is None:
+            return None, None, None, None, None, None
         _once("layer_norm")
         x, stat, kept, w = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]

@@ -38,6 +38,25 @@ def test_forward_mode_derivatives_are_refused(no_kernels, grad):
                 ops.linear8(d, m.requires_grad_(True))
 
 
+@pytest.mark.parametrize("function", ["_Act8", "_LayerNorm"])
+def test_no_gradients_are_made_for_the_8_bit_forms(no_kernels, monkeypatch, function):
+    """With out8 a layer's codes and steps are outputs without a gradient: autograd must not fill zeros of their size for the backward pass."""
+    seen = []
+    original = getattr(ops, function)
+
+    class Spy(original):
+        @staticmethod
+        def backward(ctx, *grads):
+            seen.append(grads)
+            return original.backward(ctx, *grads)
+
+    monkeypatch.setattr(ops, function, Spy)
+    x = torch.randn(4, 64, requires_grad=True)
+    y, ck = ops.act8(x, "gelu", out8=True) if function == "_Act8" else ops.layer_norm(x, out8=True)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    assert len(seen) == 1 and seen[0][0] is not None and seen[0][1:] == (None, None)
+
+
 def test_linear8_backward_keeps_its_type_under_autocast():
     """The engine carries the caller's autocast state into the backward pass (here the CPU's, with frozen parameters: no kernel is reached)."""
     x, w, g = torch.randn(5, 64, requires_grad=True), torch.randn(8, 64), torch.randn(5, 8)
