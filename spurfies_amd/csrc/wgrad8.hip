@@ -290,34 +290,38 @@ wgrad8_kernel(wgrad8_args a) {
         write((_Float16*)a.dw, (_Float16*)a.db);
 }
 
-// out[i] (+)= sum over the splits: eight threads share them, each takes every eighth in order
+// out[i] (+)= sum over the splits: eight threads share them, each takes every eighth in order.  A workgroup adds 128 outputs at a time; it walks over them, as a grid with
+// one for each would pass a launch's 2^32 threads at 2^31 outputs.
+constexpr long long REDUCE_GROUPS = 1 << 22;
 template <typename W>
 __global__ void __launch_bounds__(256)
 wgrad8_reduce_kernel(const float* __restrict__ tiles, int splits, long long count, W* dw, const float* __restrict__ bias_tiles, int n, W* db, int add) {
     __shared__ float part[8][128];
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const long long groups = (count + 127) / 128;
-    const bool is_bias = blockIdx.x >= groups;                              // the last workgroups add db
-    const long long first = (is_bias ? (long long)blockIdx.x - groups : (long long)blockIdx.x) * 128, c = first + 4 * lane;
-    const long long len = is_bias ? n : count;
-    const float* src = is_bias ? bias_tiles : tiles;
-    float s[4] = {};
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, at = threadIdx.x;
+    const long long groups = (count + 127) / 128, all = groups + (db ? (n + 127) / 128 : 0);       // the last ones add db
+    for (long long group = blockIdx.x; group < all; group += gridDim.x) {
+        const bool is_bias = group >= groups;
+        const long long first = (is_bias ? group - groups : group) * 128, c = first + 4 * lane, len = is_bias ? n : count;
+        const float* src = is_bias ? bias_tiles : tiles;
+        float s[4] = {};
 #pragma unroll 8
-    for (int i = k; i < splits; i += 8) {
-        const vec_t<float> v = load_vec(src + (size_t)i * len + c, len - c);
+        for (int i = k; i < splits; i += 8) {
+            const vec_t<float> v = load_vec(src + (size_t)i * len + c, len - c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] += v[j];
+            for (int j = 0; j < 4; ++j) s[j] += v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[k][4 * lane + j] = s[j];
+        __syncthreads();
+        if (at < 128 && first + at < len) {
+            float t = part[0][at];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) t += part[i][at];
+            W* out = (is_bias ? db : dw) + first + at;
+            *out = (W)(add ? (float)*out + t : t);
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) part[k][4 * lane + j] = s[j];
-    __syncthreads();
-    const int at = threadIdx.x;
-    if (at >= 128 || first + at >= len) return;
-    float t = part[0][at];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) t += part[i][at];
-    W* out = (is_bias ? db : dw) + first + at;
-    *out = (W)(add ? (float)*out + t : t);
 }
 
 constexpr int STAGE = 32;
@@ -414,7 +418,7 @@ int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, c
     else if (type == SPF_TYPE_BF16) launch<__bf16>(a, p, is_plain, s);
     else launch<_Float16>(a, p, is_plain, s);
     if (!direct) {
-        const int64_t groups = (n * cols + 127) / 128 + (db ? (n + 127) / 128 : 0);
+        const int64_t all = (n * cols + 127) / 128 + (db ? (n + 127) / 128 : 0), groups = all < REDUCE_GROUPS ? all : REDUCE_GROUPS;
         const auto reduce = [&](auto* w, auto* b) { wgrad8_reduce_kernel<<<(unsigned)groups, 256, 0, s>>>(workspace, p.splits, n * cols, w, bias_tiles, (int)n, b, accumulate); };
         if (wtype == SPF_TYPE_F32) reduce((float*)dw, (float*)db);
         else if (wtype == SPF_TYPE_BF16) reduce((__bf16*)dw, (__bf16*)db);

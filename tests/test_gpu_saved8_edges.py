@@ -143,3 +143,27 @@ def test_linear8_keeps_its_type_where_the_backward_pass_runs_under_autocast(dtyp
         with torch.autocast("cuda", dtype=other):
             got = torch.autograd.grad(ops.linear8(x, w, b), (x, w, b), g)
         assert all(p.dtype == dtype and torch.equal(p, q) for p, q in zip(got, want))
+
+
+# ---- sizes beyond a launch's 2^32 work-items --------------------------------------------------------------------------------------------
+def _room(gigabytes):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gigabytes * 1e9:
+        pytest.skip(f"needs {gigabytes} GB of GPU memory")
+
+
+def test_wgrad8_adds_into_more_than_2_31_outputs():
+    from spurfies_amd import ops
+
+    _room(24)
+    n, k = 1 << 18, 8200
+    g = randn((3, n), torch.bfloat16, 1)
+    ck = ops.checkpoint8(randn((3, k), torch.bfloat16, 2))
+    out, db = torch.ones(n, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    ops.wgrad8(g, ck, out=out, dbias=db)
+    for rows in (slice(0, 300), slice(n // 2, n // 2 + 300), slice(n - 300, n)):
+        part, dpart = torch.ones(300, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(300, dtype=torch.bfloat16, device="cuda")
+        ops.wgrad8(g[:, rows].contiguous(), ck, out=part, dbias=dpart)
+        assert torch.equal(out[rows], part) and torch.equal(db[rows], dpart)
+    del out, part
+    torch.cuda.empty_cache()
