@@ -167,3 +167,42 @@ def test_wgrad8_adds_into_more_than_2_31_outputs():
         assert torch.equal(out[rows], part) and torch.equal(db[rows], dpart)
     del out, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_of_many_wide_rows(dtype):
+    """The widest form's rows come out as they do in small batches."""
+    from spurfies_amd import ops
+
+    rows, cols = 16384 + 37, 16385
+    x = randn((64, cols), dtype, 1)
+    big = x.repeat(-(-rows // 64), 1)[:rows]
+    w, b = randn((cols,), dtype, 2), randn((cols,), dtype, 3)
+    big.requires_grad_(True)
+    y = ops.layer_norm(big, w, b)
+    dx, = torch.autograd.grad(y, big, big.detach())
+    x.requires_grad_(True)
+    y0 = ops.layer_norm(x, w, b)
+    d0, = torch.autograd.grad(y0, x, x.detach())
+    for i in range(0, rows, 64):
+        n = min(64, rows - i)
+        assert torch.equal(y[i:i + n], y0[:n]) and torch.equal(dx[i:i + n], d0[:n]), i
+
+
+def test_layer_norm_of_more_than_2_22_wide_rows():
+    """Through the library, with broadcast inputs: 2^22 rows of 1024 threads each are 2^32 threads."""
+    from spurfies_amd import _lib
+
+    rows, cols = (1 << 22) + 3, 8200
+    _room(80)
+    l, s = _lib.lib(), _lib.stream_ptr()
+    x, g = randn((1, cols), torch.bfloat16, 1), randn((1, cols), torch.bfloat16, 2)
+    mean, rstd = torch.full((rows,), 0.25, device="cuda"), torch.full((rows,), 1.5, device="cuda")
+    dx, one = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda"), torch.empty(1, cols, dtype=torch.bfloat16, device="cuda")
+    for out, n in ((dx, rows), (one, 1)):
+        _lib.check(l.spf_layer_norm_backward(_lib.ptr(g), 1, 0, n, cols, _lib.ptr(x), 0, None, None, _lib.ptr(mean), _lib.ptr(rstd), None, 1, _lib.ptr(out), cols, None, None, 0,
+                                             None, s))
+    for i in (0, 1, 1 << 20, (1 << 22) - 1, 1 << 22, rows - 1):
+        assert torch.equal(dx[i], one[0]), i
+    del dx
+    torch.cuda.empty_cache()
