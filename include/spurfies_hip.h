@@ -781,8 +781,8 @@ int spf_layer_norm_forward(const void* x, int32_t type, int64_t ldx, int64_t row
                            int32_t wtype, float eps, void* y, int64_t ldy, float* mean, float* rstd, uint8_t* in_codes, uint8_t* in_steps,
                            uint8_t* out_codes, uint8_t* out_steps, void* stream);
 int64_t spf_layer_norm_workspace_floats(int64_t rows, int64_t cols);
-/* From dy and one of x and its 8-bit form (the other NULL): dx, dweight, dbias, each or NULL.  dweight / dbias [cols] of type wtype;
- * accumulate != 0 adds to them.  workspace: spf_layer_norm_workspace_floats() floats, needed for dweight / dbias.  Bit-reproducible. */
+/* From dy and one of x and its 8-bit form (the other NULL): dx, dweight, dbias, each or NULL.  dweight / dbias [cols] of type wtype (two
+ * places); accumulate != 0 adds to them.  workspace: spf_layer_norm_workspace_floats() floats, needed for dweight / dbias.  Bit-reproducible. */
 int spf_layer_norm_backward(const void* dy, int32_t type, int64_t ldd, int64_t rows, int64_t cols, const void* x, int64_t ldx,
                             const uint8_t* codes, const uint8_t* steps, const float* mean, const float* rstd, const void* weight, int32_t wtype,
                             void* dx, int64_t lddx, void* dweight, void* dbias, int32_t accumulate, float* workspace, void* stream);

@@ -541,6 +541,7 @@ int spf_layer_norm_backward(const void* dy, int32_t type, int64_t ldd, int64_t r
     if (misaligned(x, type_size(type)) || misaligned(dy, type_size(type)) || misaligned(dx, type_size(type)) || misaligned(weight, type_size(wtype)) ||
         misaligned(dweight, type_size(wtype)) || misaligned(dbias, type_size(wtype)) || misaligned(codes, 16) || misaligned(workspace, 4))
         return fail(SPF_EINVAL, "%s: misaligned pointer", who);
+    if (dweight && dweight == dbias) return fail(SPF_EINVAL, "%s: dweight and dbias are one address", who);
     if (!dx && !dweight && !dbias) return SPF_OK;
     norm_args a = {};
     a.dy = dy, a.ldd = ldd, a.rows = rows, a.cols = (int)cols, a.x = x, a.ldx = ldx, a.in_codes = (uint8_t*)codes, a.in_steps = (uint8_t*)steps;

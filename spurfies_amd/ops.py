@@ -1787,9 +1787,12 @@ def act8(x, kind, param=None, out8=False):
 
 
 def _sinks_of(needs, *params):
-    """The gradient sinks of the parameters that need a gradient, if all of those have one (else None)."""
+    """The gradient sinks of the parameters that need a gradient, if all of those have one and none is another's (else None: autograd adds the gradients up)."""
     sinks = [_sink(t) if need and t is not None else None for t, need in zip(params, needs)]
-    return sinks if any(s is not None for s in sinks) and all(s is not None or not need for s, need in zip(sinks, needs)) else None
+    places = [s.data_ptr() for s in sinks if s is not None]
+    if not places or len(set(places)) < len(places) or any(s is None and need for s, need in zip(sinks, needs)):
+        return None
+    return sinks
 
 
 def _layer_norm_forward(x, w, b, eps, train, saved8, out8):

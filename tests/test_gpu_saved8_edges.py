@@ -206,3 +206,23 @@ def test_layer_norm_of_more_than_2_22_wide_rows():
         assert torch.equal(dx[i], one[0]), i
     del dx
     torch.cuda.empty_cache()
+
+
+# ---- gradients into shared or partial places --------------------------------------------------------------------------------------------
+def test_one_parameter_as_weight_and_bias_with_a_sink():
+    """The same tensor twice: both gradients arrive in its .grad."""
+    from spurfies_amd import ops
+
+    x, g = randn((500, 96), torch.float32, 1), randn((500, 96), torch.float32, 2)
+    p = randn((96,), torch.float32, 3).requires_grad_(True)
+    q, r = p.detach().clone().requires_grad_(True), p.detach().clone().requires_grad_(True)
+    dq, dr = torch.autograd.grad(ops.layer_norm(x, q, r), (q, r), g)
+    p.grad = torch.full_like(p, 0.5)
+    ops.set_grad_sinks([p])
+    try:
+        ops.layer_norm(x, p, p).backward(g)
+    finally:
+        ops.set_grad_sinks([p], on=False)
+    # 0.5, dw and db added in one order or another: two roundings of sums no larger than their magnitudes'
+    want = 0.5 + f64(dq) + f64(dr)
+    close(p.grad, want, 3 * U * (0.5 + np.abs(f64(dq)) + np.abs(f64(dr))), "grad")

@@ -102,3 +102,8 @@ def test_python_refuses_bad_arguments():
     assert ck.rows == 4 and ck.nbytes == 4 * 66
     with pytest.raises(ValueError, match="GPU"):
         ck.restore()
+
+
+def test_library_refuses_one_place_for_both_parameter_gradients(lib):
+    p = ctypes.c_void_p(4096)                                              # never dereferenced
+    assert lib.spf_layer_norm_backward(p, 0, 32, 4, 32, p, 32, None, None, p, p, p, 0, None, 32, p, p, 1, p, None) == -22 and "one address" in lib.spf_last_error().decode()
