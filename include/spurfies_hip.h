@@ -794,6 +794,12 @@ int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols,
                void* dw, void* db, int32_t wtype, int32_t accumulate, float* workspace, void* stream);
 
+/* db of spf_wgrad8 by itself, the same bits, for a layer whose weight is not trained: cols as there, the saved input is not needed.
+ * workspace: spf_wgrad8_bias_workspace_floats() floats. */
+int64_t spf_wgrad8_bias_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t type);
+int spf_wgrad8_bias(const void* g, int32_t type, int64_t ldg, int64_t rows, int64_t n, int64_t cols, void* db, int32_t wtype,
+                    int32_t accumulate, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

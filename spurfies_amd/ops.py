@@ -1942,17 +1942,23 @@ def _product(a, b):
         return a @ b
 
 
+def _wgrad8_bias_into(m, ld, cols, db, accumulate):
+    rows, n = m.shape
+    ws = torch.empty(_lib.lib().spf_wgrad8_bias_workspace_floats(rows, n, cols, _TYPES[m.dtype]), dtype=torch.float32, device=m.device)
+    _lib.call("spf_wgrad8_bias", m.device, m.data_ptr(), _TYPES[m.dtype], ld, rows, n, cols, db.data_ptr(), _TYPES[db.dtype], int(accumulate), ws.data_ptr())
+
+
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, codes, steps):
         y = torch.nn.functional.linear(x, w, b)               # a plain product: the library's
-        if not any(ctx.needs_input_grad[1:3]):                # frozen parameters: dx needs the weight alone
+        if not ctx.needs_input_grad[1]:                       # a frozen weight: dx needs the weight alone, db neither
             codes = steps = None
         elif codes is None:
             ck = checkpoint8(x)
             codes, steps = ck.codes, ck.steps
         ctx.save_for_backward(w, codes, steps)
-        ctx.sinks = _sinks_of(ctx.needs_input_grad[1:3], w, b) if ctx.needs_input_grad[1] else None
+        ctx.sinks = _sinks_of(ctx.needs_input_grad[1:3], w, b)
         return y
 
     @staticmethod
@@ -1965,14 +1971,18 @@ class _Linear8(torch.autograd.Function):
         dx = _product(m, w).view(g.shape[:-1] + (cols,)) if need_x else None
         if not need_w and not need_b:
             return dx, None, None, None, None
+        dw, db = ctx.sinks if ctx.sinks is not None else (None, None)
+        if ctx.sinks is None:
+            new = torch.zeros if m.shape[0] == 0 else torch.empty
+            dw = new((n, cols), dtype=w.dtype, device=g.device) if need_w else None
+            db = new((n,), dtype=w.dtype, device=g.device) if need_b else None
+        if need_w:
+            _wgrad8_into(m, ld, codes, steps, cols, dw, db, ctx.sinks is not None)
+        else:
+            _wgrad8_bias_into(m, ld, cols, db, ctx.sinks is not None)
         if ctx.sinks is not None:
-            _wgrad8_into(m, ld, codes, steps, cols, ctx.sinks[0], ctx.sinks[1], True)
-            return dx, None, None, None, None
-        new = torch.zeros if m.shape[0] == 0 else torch.empty
-        dw = new((n, cols), dtype=w.dtype, device=g.device)
-        db = new((n,), dtype=w.dtype, device=g.device) if need_b else None
-        _wgrad8_into(m, ld, codes, steps, cols, dw, db, False)
-        return dx, (dw if need_w else None), db, None, None
+            dw = db = None
+        return dx, dw, db, None, None
 
 
 def linear8(x, weight, bias=None, saved=None):

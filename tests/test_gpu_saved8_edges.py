@@ -226,3 +226,72 @@ def test_one_parameter_as_weight_and_bias_with_a_sink():
     # 0.5, dw and db added in one order or another: two roundings of sums no larger than their magnitudes'
     want = 0.5 + f64(dq) + f64(dr)
     close(p.grad, want, 3 * U * (0.5 + np.abs(f64(dq)) + np.abs(f64(dr))), "grad")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(1, 1), (7, 3), (1000, 40), (33, 515), (70001, 256), (9, 9001)])
+def test_linear8_with_only_the_bias_to_train(dtype, rows, n):
+    """A column sum: nothing of the input is packed or kept, and no weight gradient is formed."""
+    from spurfies_amd import ops
+
+    x, w = randn((rows, 64), dtype, 1), randn((n, 64), dtype, 2, scale=0.1)
+    b = randn((n,), dtype, 3).requires_grad_(True)
+    g = randn((rows, n + 5), dtype, 4)[:, :n]
+    y = ops.linear8(x, w, b)
+    assert all(t is None or t.dtype != torch.uint8 for t in y.grad_fn.saved_tensors)
+    db, = torch.autograd.grad(y, b, g, retain_graph=True)
+    G = f64(g)
+    # a chain of at most one addition a row, 64 where splits meet, and the last rounding
+    tol = half(dtype) * np.abs(G.sum(0)) + (rows + 64) * U * np.abs(G).sum(0) + tiny(dtype)
+    assert db.dtype == dtype
+    close(db, G.sum(0), tol, "db")
+    # independent roundings: a thread's chain of at most 128 rows, the splits and their sum each leave a few u of the root of the rows
+    assert np.linalg.norm(f64(db) - G.sum(0)) < (half(dtype) + 8 * U) * np.linalg.norm(G.sum(0)) + 8 * U * np.sqrt(rows) * np.sqrt(n) + tiny(dtype)
+    # the same bits as beside a weight gradient
+    v = w.detach().clone().requires_grad_(True)
+    assert torch.equal(db, torch.autograd.grad(ops.linear8(x, v, b), (v, b), g)[1])
+    b.grad = torch.full_like(b, 2.0)
+    ops.set_grad_sinks([b])
+    try:
+        z = ops.linear8(x, w, b)
+        z.backward(g)
+    finally:
+        ops.set_grad_sinks([b], on=False)
+    close(b.grad, 2.0 + G.sum(0), half(dtype) * np.abs(2.0 + G.sum(0)) + (rows + 66) * U * (2 + np.abs(G).sum(0)) + tiny(dtype), "sink")
+
+
+def test_linear8_with_only_the_bias_to_train_in_a_captured_step():
+    from spurfies_amd import ops
+
+    x, w = randn((5000, 64), torch.float32, 1), randn((300, 64), torch.float32, 2)
+    b = randn((300,), torch.float32, 3).requires_grad_(True)
+    gs = [randn((5000, 300), torch.float32, 10 + i) for i in range(3)]
+    want = [torch.autograd.grad(ops.linear8(x, w, b), b, h)[0] for h in gs]
+    c, g = b.detach().clone().requires_grad_(True), gs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.linear8(x, w, c), c, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        db, = torch.autograd.grad(ops.linear8(x, w, c), c, g)
+    for h, d in zip(gs, want):
+        g.copy_(h)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(db, d)
+        torch.randn(1000, device="cuda").sum().item()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(300000, 256, 256), (8192, 1024, 1024), (4100, 300, 140), (40, 7, 64), (1000, 2000, 2000)])
+def test_bias_gradient_by_itself_in_every_plan(dtype, rows, n, k):
+    """Wide, middle and narrow tiles, split rows and not: the bits of the call that forms the weight gradient as well."""
+    from spurfies_amd import ops
+
+    g = randn((rows, n), dtype, 1)
+    want = ops.wgrad8(g, ops.checkpoint8(randn((rows, k), dtype, 2)))[1]
+    db = torch.empty_like(want)
+    ops._wgrad8_bias_into(g, n, k, db, False)
+    assert torch.equal(db, want)

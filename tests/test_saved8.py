@@ -107,3 +107,18 @@ def test_python_refuses_bad_arguments():
 def test_library_refuses_one_place_for_both_parameter_gradients(lib):
     p = ctypes.c_void_p(4096)                                              # never dereferenced
     assert lib.spf_layer_norm_backward(p, 0, 32, 4, 32, p, 32, None, None, p, p, p, 0, None, 32, p, p, 1, p, None) == -22 and "one address" in lib.spf_last_error().decode()
+
+
+def test_bias_gradient_by_itself_refuses_bad_arguments(lib):
+    p, q = ctypes.c_void_p(4096), ctypes.c_void_p(4096 + 2)                # never dereferenced: every call is refused on the host
+    err = lambda: lib.spf_last_error().decode()  # noqa: E731
+    sums = lambda g=p, type=0, ld=32, rows=4, n=32, k=32, db=p, wtype=0, ws=p: lib.spf_wgrad8_bias(g, type, ld, rows, n, k, db, wtype, 0, ws, None)  # noqa: E731
+    for call, why in ((lambda: sums(type=3), "type"), (lambda: sums(wtype=-1), "type"), (lambda: sums(rows=-1), "negative"), (lambda: sums(n=1 << 21), "2^20"),
+                      (lambda: sums(g=None), "null"), (lambda: sums(db=None), "null"), (lambda: sums(ws=None), "null"), (lambda: sums(ld=-1), "stride"), (lambda: sums(g=q), "misaligned"),
+                      (lambda: sums(db=q), "misaligned")):
+        assert call() == -22 and why in err()
+    for rows, n in ((0, 32), (4, 0)):
+        assert sums(g=None, rows=rows, n=n, db=None, ws=None) == 0 and lib.spf_wgrad8_bias_workspace_floats(rows, n, 32, 0) == 0
+    for rows, n, k in ((1, 1, 1), (70001, 256, 64), (9, 9001, 64), (1 << 30, 1 << 10, 1 << 10)):
+        w = lib.spf_wgrad8_bias_workspace_floats(rows, n, k, 1)
+        assert w % n == 0 and w >= n and (k + 1) * w == lib.spf_wgrad8_workspace_floats(rows, n, k, 1, 1)

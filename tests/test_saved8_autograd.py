@@ -64,3 +64,11 @@ def test_linear8_backward_keeps_its_type_under_autocast():
     with torch.autocast("cpu", dtype=torch.bfloat16):
         dx, = torch.autograd.grad(y, x, g)
     assert dx.dtype == torch.float32 and torch.equal(dx, g @ w)
+
+
+def test_linear8_with_only_the_bias_to_train_saves_nothing_of_the_input(no_kernels):
+    x, w, b = torch.randn(5, 64), torch.randn(8, 64), torch.randn(8, requires_grad=True)
+    y = ops.linear8(x, w, b)
+    assert not no_kernels and all(t is None or t.dtype != torch.uint8 for t in y.grad_fn.saved_tensors)
+    y.backward(torch.ones_like(y))
+    assert [c[0] for c in no_kernels] == ["spf_wgrad8_bias"]
