@@ -788,8 +788,9 @@ int spf_layer_norm_backward(const void* dy, int32_t type, int64_t ldd, int64_t r
                             void* dx, int64_t lddx, void* dweight, void* dbias, int32_t accumulate, float* workspace, void* stream);
 
 /* dw [n][cols] = g^T a and db [n] (or NULL) = column sums of g, for g [rows][n] and a [rows][cols] in its 8-bit form: the weight and bias
- * gradient of a linear layer.  Products are exact, sums fp32, one rounding to wtype; accumulate != 0 adds to dw / db.  A row of g or a
- * block of a that is not finite gives NaN.  Large products need ldg below 64 MB.  workspace: spf_wgrad8_workspace_floats() floats.  Bit-reproducible. */
+ * gradient of a linear layer.  Products are exact, sums fp32, one rounding to wtype; accumulate != 0 adds to dw / db.  A column of g that is
+ * not finite makes its row of dw not finite (db is the column's sum: an infinity stays one), a block of a that is not finite gives NaN.  Large
+ * products need ldg below 64 MB.  workspace: spf_wgrad8_workspace_floats() floats.  Bit-reproducible. */
 int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t type, int32_t accumulate);
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols,
                void* dw, void* db, int32_t wtype, int32_t accumulate, float* workspace, void* stream);

@@ -295,3 +295,20 @@ def test_bias_gradient_by_itself_in_every_plan(dtype, rows, n, k):
     db = torch.empty_like(want)
     ops._wgrad8_bias_into(g, n, k, db, False)
     assert torch.equal(db, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(33, 40), (40, 5), (64, 260), (70001, 128)])
+def test_wgrad8_bias_gradient_of_infinities(dtype, rows, n):
+    """db is the column's sum: an infinity stays one, in whichever row it is; both signs together, or a NaN, give NaN.  The weight gradient is not finite there."""
+    from spurfies_amd import ops
+
+    inf, nan = float("inf"), float("nan")
+    ck = ops.checkpoint8(randn((rows, 70), dtype, 1))
+    for m in (0, 5, 31, 32, rows - 2, rows - 1):
+        g = randn((rows, n), dtype, 2)
+        g[m, 0], g[m, 1], g[m, 2], g[m - 1, 2], g[m, n - 1] = inf, -inf, inf, -inf, nan
+        dw, db = ops.wgrad8(g, ck)
+        db = f64(db)
+        assert db[0] == inf and db[1] == -inf and np.isnan(db[2]) and np.isnan(db[n - 1]) and np.isfinite(db[3:n - 1]).all(), m
+        assert not torch.isfinite(dw[[0, 1, 2, n - 1]]).any() and torch.isfinite(dw[3:n - 1]).all()
