@@ -1620,6 +1620,12 @@ def _same_device(who, first, *others):
             raise ValueError(f"{who}: tensors on different devices: {first.device} and {t.device}")
 
 
+def _share(a, b):
+    """Whether two contiguous tensors overlap in memory."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
+
+
 class Checkpoint8:
     """A matrix of activations in 8 bits (include/spurfies_hip.h: spf_saved8_pack): codes [rows, 32 * blocks] and steps [rows, blocks], uint8.
     Blocks of 32 columns share a power-of-two step; an element is a sign and a magnitude of seven bits, off by at most half a step (a 127th of
@@ -1925,6 +1931,8 @@ def wgrad8(g, saved, out=None, dbias=None, bias=True):
                 raise ValueError(f"wgrad8: out / dbias must be contiguous, of one type and of the shapes {(n, saved.cols)} / {(n,)}")
     _same_device("wgrad8", g, saved.codes, out, dbias)
     if out is not None:
+        if dbias is not None and _share(out, dbias):
+            raise ValueError("wgrad8: out and dbias share memory")
         _wgrad8_into(m, ld, saved.codes, saved.steps, saved.cols, out, dbias, True)
         return out, dbias
     new = torch.zeros if rows == 0 else torch.empty

@@ -72,3 +72,11 @@ def test_linear8_with_only_the_bias_to_train_saves_nothing_of_the_input(no_kerne
     assert not no_kernels and all(t is None or t.dtype != torch.uint8 for t in y.grad_fn.saved_tensors)
     y.backward(torch.ones_like(y))
     assert [c[0] for c in no_kernels] == ["spf_wgrad8_bias"]
+
+
+def test_wgrad8_refuses_results_that_share_memory(no_kernels):
+    ck = ops.Checkpoint8(torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.uint8), 1)
+    out = torch.zeros(8, 1)
+    with pytest.raises(ValueError, match="share"):
+        ops.wgrad8(torch.zeros(4, 8), ck, out=out, dbias=out.view(8))
+    assert not no_kernels
