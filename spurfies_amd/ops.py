@@ -1934,6 +1934,7 @@ def wgrad8(g, saved, out=None, dbias=None, bias=True):
         if dbias is not None and _share(out, dbias):
             raise ValueError("wgrad8: out and dbias share memory")
         _wgrad8_into(m, ld, saved.codes, saved.steps, saved.cols, out, dbias, True)
+        torch.autograd.graph.increment_version([t for t in (out, dbias) if t is not None])         # (graphs that saved them notice)
         return out, dbias
     new = torch.zeros if rows == 0 else torch.empty
     dw = new((n, saved.cols), dtype=torch.float32, device=g.device)

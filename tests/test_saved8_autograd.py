@@ -80,3 +80,15 @@ def test_wgrad8_refuses_results_that_share_memory(no_kernels):
     with pytest.raises(ValueError, match="share"):
         ops.wgrad8(torch.zeros(4, 8), ck, out=out, dbias=out.view(8))
     assert not no_kernels
+
+
+def test_wgrad8_marks_what_it_adds_into_as_changed(no_kernels):
+    """A graph that saved the tensor before has to notice."""
+    ck = ops.Checkpoint8(torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.uint8), 32)
+    out, db, t = torch.zeros(8, 32), torch.zeros(8), torch.ones(8, 32, requires_grad=True)
+    y = (out * t).sum() + (db * t[:, 0]).sum()
+    before = out._version, db._version
+    ops.wgrad8(torch.zeros(4, 8), ck, out=out, dbias=db)
+    assert out._version > before[0] and db._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
