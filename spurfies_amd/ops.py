@@ -1590,6 +1590,8 @@ def _type_of(t, who):
 
 def _rows_of(t, who):
     """t as rows of consecutive elements: (2-D tensor, row stride); a view wherever the strides allow it."""
+    if t.is_neg():                                            # a lazily negated view (the imaginary part of a conjugate): its memory holds the other sign
+        t = t.resolve_neg()
     if t.dim() == 2 and t.is_contiguous() and t.numel() > 0:
         return t, t.shape[1]
     if t.dim() == 0:
@@ -1880,8 +1882,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
     params = [t for t in (weight, bias) if t is not None]
     for t in params:
         _type_of(t, "layer_norm")
-        if t.shape != x.shape[-1:] or not t.is_contiguous():
-            raise ValueError(f"layer_norm: weight and bias must be contiguous and of the shape {tuple(x.shape[-1:])}, got {tuple(t.shape)}")
+        if t.shape != x.shape[-1:] or not t.is_contiguous() or t.is_neg():
+            raise ValueError(f"layer_norm: weight and bias must be contiguous (and not lazily negated) and of the shape {tuple(x.shape[-1:])}, got {tuple(t.shape)}")
         if t.dtype != params[0].dtype or t.dtype not in (x.dtype, torch.float32):
             raise ValueError("layer_norm: weight and bias share one type, x's or float32")
     _same_device("layer_norm", x, *params)
@@ -1927,8 +1929,8 @@ def wgrad8(g, saved, out=None, dbias=None, bias=True):
     for t, shape in ((out, (n, saved.cols)), (dbias, (n,))):
         if t is not None:
             _type_of(t, "wgrad8")
-            if tuple(t.shape) != shape or not t.is_contiguous() or t.dtype != out.dtype:
-                raise ValueError(f"wgrad8: out / dbias must be contiguous, of one type and of the shapes {(n, saved.cols)} / {(n,)}")
+            if tuple(t.shape) != shape or not t.is_contiguous() or t.is_neg() or t.dtype != out.dtype:
+                raise ValueError(f"wgrad8: out / dbias must be contiguous (and not lazily negated), of one type and of the shapes {(n, saved.cols)} / {(n,)}")
     _same_device("wgrad8", g, saved.codes, out, dbias)
     if out is not None:
         if dbias is not None and _share(out, dbias):

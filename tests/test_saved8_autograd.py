@@ -92,3 +92,23 @@ def test_wgrad8_marks_what_it_adds_into_as_changed(no_kernels):
     assert out._version > before[0] and db._version > before[1]
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_rows_of_lazily_negated_tensors():
+    """torch's imaginary part of a conjugate is a view whose memory holds the other sign."""
+    x = torch.randn(4, 32)
+    z = torch.complex(x, -x).conj()
+    for t in (z.imag, torch._neg_view(x), torch._neg_view(x)[:, :1], torch._neg_view(x)[0]):
+        assert t.is_neg()
+        m, ld = ops._rows_of(t, "test")
+        assert not m.is_neg() and torch.equal(m, t.reshape(-1, t.shape[-1]).clone())
+        assert torch.equal(torch.as_strided(m, m.shape, (ld, 1), m.storage_offset()), m)
+
+
+def test_lazily_negated_parameters_and_results_are_refused(no_kernels):
+    x, w, ck = torch.randn(4, 32), torch.randn(32), ops.Checkpoint8(torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.uint8), 32)
+    with pytest.raises(ValueError, match="negated"):
+        ops.layer_norm(x, torch._neg_view(w))
+    with pytest.raises(ValueError, match="negated"):
+        ops.wgrad8(x, ck, out=torch._neg_view(torch.zeros(32, 32)))
+    assert not no_kernels
