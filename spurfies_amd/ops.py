@@ -1774,7 +1774,7 @@ def act8(x, kind, param=None, out8=False):
     number, default = _ACTS[kind]
     if param is not None and default is None:
         raise ValueError(f"act8: {kind} has no parameter")
-    param = float(default or 0.0) if param is None else float(param)
+    param = ctypes.c_float(default or 0.0 if param is None else param).value                   # as the kernels take it
     if kind == "leaky_relu" and not 0.0 <= param < float("inf"):
         raise ValueError("act8: leaky_relu needs a slope >= 0")
     if kind == "softplus" and not 0.0 < param < float("inf"):
@@ -1887,7 +1887,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
         if t.dtype != params[0].dtype or t.dtype not in (x.dtype, torch.float32):
             raise ValueError("layer_norm: weight and bias share one type, x's or float32")
     _same_device("layer_norm", x, *params)
-    eps = float(eps)
+    eps = ctypes.c_float(eps).value                            # as the kernels take it
     if not 0.0 <= eps < float("inf"):
         raise ValueError("layer_norm: eps must be finite and not negative")
     _no_tangents("layer_norm", x, *params)

@@ -112,3 +112,14 @@ def test_lazily_negated_parameters_and_results_are_refused(no_kernels):
     with pytest.raises(ValueError, match="negated"):
         ops.wgrad8(x, ck, out=torch._neg_view(torch.zeros(32, 32)))
     assert not no_kernels
+
+
+def test_parameters_beyond_the_kernels_32_bits_are_wrong_arguments(no_kernels):
+    x = torch.randn(4, 32)
+    for call in (lambda: ops.act8(x, "softplus", 1e-60), lambda: ops.act8(x, "softplus", 1e60), lambda: ops.act8(x, "leaky_relu", 1e60), lambda: ops.layer_norm(x, eps=1e60)):
+        with pytest.raises(ValueError):
+            call()
+    assert not no_kernels
+    ops.layer_norm(x, eps=torch.tensor(1e-5))
+    ops.act8(x, "leaky_relu", 1)
+    assert len(no_kernels) == 2
