@@ -792,6 +792,8 @@ int spf_layer_norm_backward(const void* dy, int32_t type, int64_t ldd, int64_t r
  * not finite makes its row of dw not finite (db is the column's sum: an infinity stays one), a block of a that is not finite gives NaN.  Large
  * products need ldg below 64 MB.  workspace: spf_wgrad8_workspace_floats() floats.  Bit-reproducible. */
 int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32_t type, int32_t accumulate);
+/* the width of the tiles that spf_wgrad8 takes for these sizes: 256, 128 or 64 (0: nothing to do, or refused) */
+int32_t spf_wgrad8_tile(int64_t rows, int64_t n, int64_t cols, int32_t type);
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols,
                void* dw, void* db, int32_t wtype, int32_t accumulate, float* workspace, void* stream);
 

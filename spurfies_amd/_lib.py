@@ -137,6 +137,7 @@ SIGNATURES = {
     "spf_layer_norm_workspace_floats": (C.c_int64, [_L, _L]),
     "spf_layer_norm_backward": (C.c_int, [_P, _I, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _P, _L, _P, _P, _I, _P, _P]),
     "spf_wgrad8_workspace_floats": (C.c_int64, [_L, _L, _L, _I, _I]),
+    "spf_wgrad8_tile": (_I, [_L, _L, _L, _I]),
     "spf_wgrad8_bias_workspace_floats": (C.c_int64, [_L, _L, _L, _I]),
     "spf_wgrad8_bias": (C.c_int, [_P, _I, _L, _L, _L, _L, _P, _I, _I, _P, _P]),
     "spf_wgrad8": (C.c_int, [_P, _I, _L, _P, _P, _L, _L, _L, _P, _P, _I, _I, _P, _P]),

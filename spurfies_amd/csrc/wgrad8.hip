@@ -440,6 +440,11 @@ int64_t spf_wgrad8_workspace_floats(int64_t rows, int64_t n, int64_t cols, int32
     return splits > 1 || accumulate ? splits * n * (cols + 1) : 0;
 }
 
+int32_t spf_wgrad8_tile(int64_t rows, int64_t n, int64_t cols, int32_t type) {
+    if (bad_sizes(rows, n, cols) || !type_ok(type) || rows == 0 || n == 0 || cols == 0) return 0;
+    return plan_of(rows, n, cols, type).side;
+}
+
 int spf_wgrad8(const void* g, int32_t type, int64_t ldg, const uint8_t* codes, const uint8_t* steps, int64_t rows, int64_t n, int64_t cols, void* dw, void* db,
                int32_t wtype, int32_t accumulate, float* workspace, void* stream) {
     const char* who = "spf_wgrad8";

@@ -312,3 +312,88 @@ def test_wgrad8_bias_gradient_of_infinities(dtype, rows, n):
         db = f64(db)
         assert db[0] == inf and db[1] == -inf and np.isnan(db[2]) and np.isnan(db[n - 1]) and np.isfinite(db[3:n - 1]).all(), m
         assert not torch.isfinite(dw[[0, 1, 2, n - 1]]).any() and torch.isfinite(dw[3:n - 1]).all()
+
+
+# ---- every form of the kernels ----------------------------------------------------------------------------------------------------------
+def tile(rows, n, k, dtype):
+    from spurfies_amd import _lib, ops
+
+    return _lib.lib().spf_wgrad8_tile(rows, n, k, ops._TYPES[dtype])
+
+
+# split rows and not, tiles that the layer does not fill: a last piece of one and of seven columns, rows that do not fill a stage
+WIDE = [(389017, 256, 256), (5000, 2049, 2051), (5003, 2055, 2050), (1900, 4091, 4085)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", WIDE)
+def test_wgrad8_with_the_widest_tiles(dtype, rows, n, k):
+    from spurfies_amd import ops
+
+    assert tile(rows, n, k, dtype) == 256
+    a, g = randn((rows, k), dtype, 1), randn((rows, n), dtype, 2)
+    ck = ops.checkpoint8(a)
+    dw, db = ops.wgrad8(g, ck)
+    A, G = ck.restore(torch.float32).double(), g.double()
+    want, sums = f64(G.t() @ A), f64(G.sum(0))
+    # independent roundings of a chain of three piece products a row (each up to 2 u of sums of about the root of the rows), held to eight times their spread
+    close(dw, want, 8 * 2 * U * np.sqrt(3 * rows) * np.sqrt(rows) * 2, "dw")
+    close(db, sums, 8 * U * rows * 2, "db")
+    assert np.linalg.norm(f64(dw) - want) < 2 * U * 8 * np.sqrt(3 * rows + 64) * np.linalg.norm(want)
+    assert all(torch.equal(p, q) for p, q in zip((dw, db), ops.wgrad8(g, ck)))
+    out, dbias = torch.ones_like(dw), torch.ones_like(db)
+    ops.wgrad8(g, ck, out=out, dbias=dbias)
+    assert torch.equal(out, 1 + dw) and torch.equal(dbias, 1 + db)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(5000, 2049, 2051), (1900, 4091, 4085)])
+def test_wgrad8_with_the_widest_tiles_is_exact_for_whole_numbers(dtype, rows, n, k):
+    """Sums within 24 bits do not round: every piece of every element has to arrive in its place."""
+    from spurfies_amd import ops
+
+    assert tile(rows, n, k, dtype) == 256
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    ints = lambda low, high, *shape: torch.randint(low, high, shape, generator=gen, device="cuda").double()  # noqa: E731
+    A = ints(0, 2, rows, k) * 2 - 1
+    if dtype == torch.float32:
+        G = torch.zeros(rows, n, dtype=torch.float64, device="cuda")       # one number of 23 bits a column
+        G[torch.randint(0, rows, (n,), generator=gen, device="cuda"), torch.arange(n, device="cuda")] = ints(2 ** 22, 2 ** 23, n)
+    else:
+        bits = 8 if dtype == torch.bfloat16 else 11                        # 5000 * 2047 < 2^24
+        G = ints(1 - 2 ** bits, 2 ** bits, rows, n)
+    a, g = A.to(dtype), G.to(dtype)
+    assert torch.equal(a.double(), A) and torch.equal(g.double(), G)
+    dw, db = ops.wgrad8(g, ops.checkpoint8(a))
+    assert torch.equal(dw.double(), G.t() @ A) and torch.equal(db.double(), G.sum(0))
+
+
+@pytest.mark.parametrize("saved8", [False, True])
+@pytest.mark.parametrize("dtype,rows,cols", [(torch.float32, 2003, 1030), (torch.float32, 2003, 4099), (torch.float32, 2003, 8192), (torch.bfloat16, 4001, 1500), (torch.bfloat16, 4001, 4096),
+                                             (torch.float16, 2003, 8191), (torch.float32, 150, 9001), (torch.bfloat16, 150, 9001), (torch.bfloat16, 150, 17003)])
+def test_layer_norm_of_many_rows_of_several_waves(dtype, rows, cols, saved8):
+    """Workgroups that walk over rows whose threads meet in LDS, and the column sums of rows that are read again: each row as it comes out alone, the columns as in 64 bits."""
+    from spurfies_amd import ops
+
+    x = randn((rows, cols), dtype, cols, scale=1.5, shift=0.7).requires_grad_(True)
+    w, b = randn((cols,), dtype, 1, scale=0.3, shift=1.0).requires_grad_(True), randn((cols,), dtype, 2).requires_grad_(True)
+    g = randn((rows, cols), dtype, 3)
+    y, ck = ops.layer_norm(x, w, b, saved8=saved8, out8=True)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), torch.autograd.grad(y, (x, w, b), g)))
+    assert torch.equal(ck.codes, ops.checkpoint8(y).codes) and torch.equal(ck.steps, ops.checkpoint8(y).steps)
+    for i in range(0, rows, 50):                                            # (a batch of 50 rows has a workgroup for each)
+        v = x[i:i + 50].detach().requires_grad_(True)
+        z = ops.layer_norm(v, w.detach(), b.detach(), saved8=saved8)
+        assert torch.equal(z, y[i:i + 50]) and torch.equal(torch.autograd.grad(z, v, g[i:i + 50])[0], dx[i:i + 50]), i
+    X, G = x.detach().double(), g.double()
+    R = ops.checkpoint8(x).restore(torch.float32).double() if saved8 else X
+    mean = X.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((X - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    n = (R - mean) * rstd
+    # the mean and the deviation from chains of K roundings, n from those; the columns from chains of at most rows / 16 + 64
+    K, L = 32 + cols / 2048, 64 + rows / 16
+    dmean = K * U * X.abs().mean(1, keepdim=True)
+    dn = (dmean + U * (R - mean).abs()) * rstd + n.abs() * (K * U + 2 * (dmean + U * (X - mean).abs().mean(1, keepdim=True)) * rstd + 4 * U)
+    for got, want, size, what in ((dw, (G * n).sum(0), L * U * (G * n).abs().sum(0) + (G.abs() * dn).sum(0), "dw"), (db, G.sum(0), L * U * G.abs().sum(0), "db")):
+        close(got, f64(want), half(dtype) * np.abs(f64(want)) + f64(size) + tiny(dtype), what)

@@ -122,3 +122,10 @@ def test_bias_gradient_by_itself_refuses_bad_arguments(lib):
     for rows, n, k in ((1, 1, 1), (70001, 256, 64), (9, 9001, 64), (1 << 30, 1 << 10, 1 << 10)):
         w = lib.spf_wgrad8_bias_workspace_floats(rows, n, k, 1)
         assert w % n == 0 and w >= n and (k + 1) * w == lib.spf_wgrad8_workspace_floats(rows, n, k, 1, 1)
+
+
+def test_tile_query(lib):
+    """The plan as tests see it: by sizes and type alone, nothing for what is refused."""
+    assert lib.spf_wgrad8_tile(8192, 4096, 4096, 1) == 256 and lib.spf_wgrad8_tile(1, 1, 1, 0) == 64
+    assert {lib.spf_wgrad8_tile(m, n, k, t) for m in (40, 4000, 400000) for n in (7, 100, 256, 2000) for k in (7, 100, 256, 2000) for t in (0, 1, 2)} == {64, 128, 256}
+    assert lib.spf_wgrad8_tile(0, 8, 8, 0) == lib.spf_wgrad8_tile(8, 8, 8, 7) == lib.spf_wgrad8_tile(8, 1 << 21, 8, 0) == 0
