@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(1024)
 norm_columns_kernel(const float* __restrict__ lines, int groups, int line, int cols, W* dw, W* db, int add) {
     __shared__ float part[16][64];
     const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, which = blockIdx.y;
-    const int c = blockIdx.x * 64 + lane;
+    const int c = (blockIdx.z * gridDim.x + blockIdx.x) * 64 + lane;
     W* out = which ? db : dw;
     if (!out) return;                              // the same for the whole workgroup
     float s = 0.f;
@@ -418,8 +418,11 @@ norm_columns_kernel(const float* __restrict__ lines, int groups, int line, int c
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
-// A workgroup a row, in two dimensions: a launch has less than 2^32 threads in each, which are 2^22 rows of 1024.  (Workgroups that walk over rows instead take 8 - 13 % longer.)
-dim3 wide_grid(int64_t rows) { return rows < (1 << 20) ? dim3((unsigned)rows) : dim3(1 << 20, (unsigned)((rows + (1 << 20) - 1) >> 20)); }
+// Workgroups of 1024 threads in two dimensions of the grid: a launch has less than 2^32 threads in each, which are 2^22 workgroups.  (Workgroups that walk over the rows instead
+// take 8 - 13 % longer.)
+constexpr int64_t ACROSS = 1 << 20;
+dim3 wide_grid(int64_t rows) { return dim3((unsigned)(rows < ACROSS ? rows : ACROSS), (unsigned)((rows + ACROSS - 1) / ACROSS)); }
+dim3 columns_grid(int64_t cols) { const dim3 d = wide_grid((cols + 63) / 64); return dim3(d.x, 2, d.y); }
 // f(threads a row, vectors a thread): the smallest shape whose registers hold the row
 template <typename T, bool BACKWARD, typename F> void by_width(int cols, F f) {
     constexpr int V = VEC<T>;
@@ -487,7 +490,7 @@ template <typename T, typename W, bool SAVED8> int backward_groups(const norm_ar
 template <typename T, typename W> void backward(const norm_args& a, void* dweight, void* dbias, int add, hipStream_t s) {
     const int groups = a.in_codes ? backward_groups<T, W, true>(a, s) : backward_groups<T, W, false>(a, s);
     if (a.lines)
-        norm_columns_kernel<W><<<dim3((unsigned)((a.cols + 63) / 64), 2), 1024, 0, s>>>(a.lines, groups, a.line, a.cols, (W*)dweight, (W*)dbias, add);
+        norm_columns_kernel<W><<<columns_grid(a.cols), 1024, 0, s>>>(a.lines, groups, a.line, a.cols, (W*)dweight, (W*)dbias, add);
 }
 
 // the parameters have the rows' type or fp32

@@ -208,6 +208,24 @@ def test_layer_norm_of_more_than_2_22_wide_rows():
     torch.cuda.empty_cache()
 
 
+def test_layer_norm_parameter_gradients_of_more_than_2_28_columns():
+    """Each column's sum, the last ones' too: 64 columns a workgroup of 1024 threads are a launch's 2^32 threads at 2^28."""
+    from spurfies_amd import _lib
+
+    cols = (1 << 28) + 1000
+    _room(12)
+    l, s = _lib.lib(), _lib.stream_ptr()
+    x, g = torch.randint(-3, 4, (cols,), device="cuda").float()[None], torch.randint(-3, 4, (cols,), device="cuda").float()[None]
+    mean, rstd = torch.full((1,), 1.0, device="cuda"), torch.full((1,), 0.5, device="cuda")
+    dw, db = torch.full((cols,), 9.0, device="cuda"), torch.full((cols,), 9.0, device="cuda")
+    ws = torch.empty(l.spf_layer_norm_workspace_floats(1, cols), device="cuda")
+    _lib.check(l.spf_layer_norm_backward(_lib.ptr(g), 0, cols, 1, cols, _lib.ptr(x), cols, None, None, _lib.ptr(mean), _lib.ptr(rstd), None, 0, None, cols, _lib.ptr(dw), _lib.ptr(db), 0,
+                                         _lib.ptr(ws), s))
+    assert torch.equal(db, g[0]) and torch.equal(dw, (g * ((x - 1) * 0.5))[0])               # small whole numbers and halves: nothing rounds
+    del ws
+    torch.cuda.empty_cache()
+
+
 # ---- gradients into shared or partial places --------------------------------------------------------------------------------------------
 def test_one_parameter_as_weight_and_bias_with_a_sink():
     """The same tensor twice: both gradients arrive in its .grad."""
