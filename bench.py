@@ -537,17 +537,25 @@ def main_eval(args):
         torch.distributed.destroy_process_group()
 
 
+# sources of operators that the measured steps do not run (training operators with 8-bit saved activations; last section of the header)
+OTHER_SOURCES = ("act8.hip", "norm.hip", "saved8.h", "wgrad8.hip")
+OTHER_SECTION = " * Training operators of normalised MLP layers"
+
+
 def csrc_digest():
-    """sha256 over the library's sources (spurfies_amd/csrc/*, include/spurfies_hip.h) and its compiler flags: the identity of the KERNEL code of this tree.  The
-    counter / power collections under profiles/ record it (tools/pmc_traffic.py, tools/power_probe.py); a collection whose digest differs from
-    the running tree's is stale evidence and is not quoted."""
+    """sha256 over the sources of the measured steps' kernels (spurfies_amd/csrc/*, include/spurfies_hip.h, both without OTHER_SOURCES) and the compiler flags: the
+    identity of the KERNEL code behind this bench's figures.  The counter / power collections under profiles/ record it (tools/pmc_traffic.py,
+    tools/power_probe.py); a collection whose digest differs from the running tree's is stale evidence and is not quoted."""
     import hashlib
 
     h = hashlib.sha256()
-    files = sorted(os.path.join(ROOT, "spurfies_amd", "csrc", f) for f in os.listdir(os.path.join(ROOT, "spurfies_amd", "csrc")))
-    for path in files + [os.path.join(ROOT, "include", "spurfies_hip.h")]:
-        h.update(os.path.basename(path).encode())
-        h.update(open(path, "rb").read())
+    folder = os.path.join(ROOT, "spurfies_amd", "csrc")
+    for name in sorted(os.listdir(folder)):
+        if name not in OTHER_SOURCES:
+            h.update(name.encode())
+            h.update(open(os.path.join(folder, name), "rb").read())
+    h.update(b"spurfies_hip.h")
+    h.update(open(os.path.join(ROOT, "include", "spurfies_hip.h"), "rb").read().split(OTHER_SECTION.encode())[0])
     from spurfies_amd import build as _build
 
     h.update(" ".join(_build.FLAGS).encode())          # the compiler flags are part of the kernels' identity (round 6: -amdgpu-mfma-vgpr-form)
