@@ -6,9 +6,9 @@
 //
 // One kernel each way: a pass over rows of 32-column blocks, 16 bytes of x a lane, so 8 (fp32) or 4 (16-bit types) lanes share a block and find its
 // largest magnitude with two or three moves of the vector pipe — no LDS, no second read.  Bound by HBM; the arithmetic (about 8 vector instructions
-// an element for the bytes, 15 for GELU) stays under the loads of other waves.  Each thread has four blocks in flight.
-// Measured on MI355X: 389017 x 256 fp32, LeakyReLU, 148 us forward and 163 back (6.1 and 5.5 TB/s); 16384 x 8192 bf16, GELU, 119 and 145 (5.7 and 4.6 TB/s; 139 and 192
-// with the library's erf and exp); 389017 x 104 fp32 packed in 36 us and restored in 32.
+// an element for the bytes, 17 for GELU in 16 bits, 40 in fp32) stays under the loads of other waves, but for softplus' logarithm.  Each thread has four blocks in flight.
+// Measured on MI355X (medians): 389017 x 256 fp32, LeakyReLU, 152 us forward and 168 back (5.9 and 5.4 TB/s); 16384 x 8192 bf16, GELU, 119 and 150 (5.7 and 4.5 TB/s; 139 and
+// 192 with the library's erf and exp), fp32 211 and 220 (5.8 and 5.5 TB/s), softplus fp32 383 and 218; 389017 x 104 fp32 packed in 47 us and restored in 32.
 #include <math.h>
 
 #include "saved8.h"

@@ -5,13 +5,13 @@
 //
 // A row stays in registers from its one read to its one write: up to 16 elements a thread, so the threads a row gets follow from its width — 8 to 64
 // lanes of a wave (several rows share a wave below 256 fp32 / 512 16-bit columns), then 256, then 1024 threads.  The mean is taken before the squares (two
-// sums over the registers), so rows that sit far from zero lose nothing.  Workgroups walk over the rows with the next row's loads in flight.
+// sums over the registers), so rows that sit far from zero lose no more than the mean's own rounding.  Workgroups walk over the rows with the next row's loads in flight.
 // The weight gradients need every row: each thread keeps its columns' sums in registers over all the rows of its workgroup, the workgroup's rows
 // are added through LDS, and one line per workgroup goes to the workspace; a second launch adds the lines in a fixed order.  No atomics: the same
 // call gives the same bits.  Rows too wide for that (forward 16384, backward 8192 columns) are read again for each
 // step — they stay in the caches — with the column sums in a kernel of their own.
-// Measured on MI355X, HBM-bound: 389017 x 256 fp32 147 us forward (5.4 TB/s) and 233 + 6 back (5.1 TB/s); 16384 x 4096 bf16 saved in 8 bits 65 (5.2 TB/s) and
-// 85 + 6 (4.0 TB/s: there the barrier that every row ends in shows, at three workgroups a compute unit).
+// Measured on MI355X (medians), HBM-bound: 389017 x 256 fp32 148 us forward (5.4 TB/s) and 239 + 7 back (5.0 TB/s); 16384 x 4096 bf16 saved in 8 bits 68 (5.0 TB/s) and
+// 86 + 6 (3.9 TB/s: there the barrier that every row ends in shows, at three workgroups a compute unit); 8192 x 12288 bf16 93 (4.3 TB/s) and, read again, 331 back (1.8 TB/s).
 #include <math.h>
 
 #include "saved8.h"

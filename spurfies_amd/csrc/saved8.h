@@ -174,7 +174,8 @@ template <int N> __device__ __forceinline__ void s8_load(const uint8_t* codes, s
     }
 }
 
-// row = n / d for 0 <= n < 2^31 by one multiplication (d fixed for a launch): n / d = (mulhi(n, mul) + n) >> shift
+// row = n / d for 0 <= n < 2^31 by one multiplication (d fixed for a launch): n / d = (mulhi(n, mul) + n) >> shift (Granlund & Montgomery, Division by invariant
+// integers using multiplication, 1994)
 struct fast_div {
     uint32_t d, mul, shift;
     fast_div() = default;

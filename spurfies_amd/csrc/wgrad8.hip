@@ -11,9 +11,9 @@
 // The rows are shared out over enough workgroups to fill the chip.  Each leaves an fp32 tile in the workspace, and a second launch adds them in a
 // fixed order (no atomics: the same call gives the same bits).  db rides along: a loading thread always holds the same eight columns of G.
 //
-// Measured on MI355X: 8192 rows, 4096 x 4096, bf16: 290 us = 948 TFLOP/s (a plain bf16 product of that shape by the library: 280 us); 389017 rows, 256 x 256,
-// fp32: 159 us, of which this kernel 139 (3.6 TB/s of operands; three piece products keep the matrix pipe 49 % busy) and the sum of the splits 12; 1237 rows,
-// 131 x 515, fp16: 9 + 3 us.
+// Measured on MI355X: 8192 rows, 4096 x 4096, bf16: 251 - 272 us from box to box = 1010 - 1095 TFLOP/s (a plain bf16 product of that shape by the library, where this took
+// 251: 221 - 227 us); 389017 rows, 256 x 256, fp32: 154 us, of which this kernel 135 (3.7 TB/s of operands; three piece products keep the matrix pipe half busy) and
+// the sum of the splits 12; 1237 rows, 131 x 515, fp16: 9 + 3 us.
 #include <math.h>
 
 #include "saved8.h"
@@ -338,8 +338,8 @@ struct plan {
 // The tile and the number of row splits with the least estimated time.  A large tile reads its operands least often, but a layer that does not fill it wastes it,
 // and a workgroup with a large tile has a compute unit to itself; splits fill the chip and shorten the chain of stages, but each leaves an fp32 tile that is written
 // and read again.  The constants are microseconds on MI355X: a stage with all its compute unit's workgroups at work, a stage of a workgroup that is alone there,
-// and 5 MB of split tiles.  Measured with the tile set by hand, 256 / 128 / 64 wide: 8192 rows, 4096 x 4096: fp32 641, 797, 1203 us, bf16 288, 369, 601;
-// 389017 rows, 256 x 256, fp32: 162, 219, 358; 400000 rows, 128 x 256, fp32: 157, 109, 169; 1000 rows, 2000 x 2000, bf16: 44, 43, 28.
+// and 5 MB of split tiles.  Measured with the tile set by hand, 256 / 128 / 64 wide: 8192 rows, 4096 x 4096: fp32 621, 783, 1282 us, bf16 261, 437, 652;
+// 389017 rows, 256 x 256, fp32: 154, 180, 259; 400000 rows, 128 x 256, fp32: 137, 101, 157; 1000 rows, 2000 x 2000, bf16: 47, 25, 25.
 struct tile_kind {
     int side, resident[3];           // workgroups of a compute unit; by SPF_TYPE_*
     float busy[3], alone[3];
