@@ -1577,6 +1577,7 @@ class FusedLoss(_GradModeFunction):
 # captured steps and streams never share one.
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}             # SPF_TYPE_*
+_F32_END, _F32_ZERO = 2.0 ** 128 - 2.0 ** 103, 2.0 ** -150                    # from here up, and up to here, a double is infinity or zero in 32 bits
 _ACTS = {"leaky_relu": (0, 0.01), "softplus": (1, 1.0), "silu": (2, None), "gelu": (3, None)}      # SPF_ACT_*, the parameter's default
 
 
@@ -1702,11 +1703,10 @@ def _bytes8(rows, cols):
 
 
 def _no_tangents(who, *tensors):
-    """Refuse forward-mode derivatives: a dual tensor has a data pointer and needs no gradient, so its tangent would be dropped in silence."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{who}: there is no forward-mode derivative")
+    """Inside a forward-mode level, refuse its derivatives: a dual tensor has a data pointer and needs no gradient, so its tangent would be dropped in silence."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who}: there is no forward-mode derivative")
 
 
 def _needs_grad(*tensors):
@@ -1774,14 +1774,15 @@ def act8(x, kind, param=None, out8=False):
     number, default = _ACTS[kind]
     if param is not None and default is None:
         raise ValueError(f"act8: {kind} has no parameter")
-    param = ctypes.c_float(default or 0.0 if param is None else param).value                   # as the kernels take it
-    if kind == "leaky_relu" and not 0.0 <= param < float("inf"):
+    param = float(default or 0.0) if param is None else float(param)
+    if kind == "leaky_relu" and not 0.0 <= param < _F32_END:
         raise ValueError("act8: leaky_relu needs a slope >= 0")
-    if kind == "softplus" and not 0.0 < param < float("inf"):
+    if kind == "softplus" and not _F32_ZERO < param < _F32_END:
         raise ValueError("act8: softplus needs beta > 0")
     if x.dim() == 0:
         raise ValueError("act8: needs at least one dimension")
-    _no_tangents("act8", x)
+    if forward_ad._current_level >= 0:
+        _no_tangents("act8", x)
     if _needs_grad(x):
         r = _Act8.apply(x, number, param, bool(out8))
         if not out8:
@@ -1887,10 +1888,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, saved8=False, out8=False):
         if t.dtype != params[0].dtype or t.dtype not in (x.dtype, torch.float32):
             raise ValueError("layer_norm: weight and bias share one type, x's or float32")
     _same_device("layer_norm", x, *params)
-    eps = ctypes.c_float(eps).value                            # as the kernels take it
-    if not 0.0 <= eps < float("inf"):
+    eps = float(eps)
+    if not 0.0 <= eps < _F32_END:
         raise ValueError("layer_norm: eps must be finite and not negative")
-    _no_tangents("layer_norm", x, *params)
+    if forward_ad._current_level >= 0:
+        _no_tangents("layer_norm", x, *params)
     if _needs_grad(x, weight, bias):
         r = _LayerNorm.apply(x, weight, bias, eps, bool(saved8), bool(out8))
         if not out8:
