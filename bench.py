@@ -545,7 +545,7 @@ OTHER_SECTION = " * Training operators of normalised MLP layers"
 def csrc_digest():
     """sha256 over the sources of the measured steps' kernels (spurfies_amd/csrc/*, include/spurfies_hip.h, both without OTHER_SOURCES) and the compiler flags: the
     identity of the KERNEL code behind this bench's figures.  The counter / power collections under profiles/ record it (tools/pmc_traffic.py,
-    tools/power_probe.py); a collection whose digest differs from the running tree's is stale evidence and is not quoted (round-4 verdict item 8)."""
+    tools/power_probe.py); a collection whose digest differs from the running tree's is stale evidence and is not quoted."""
     import hashlib
 
     h = hashlib.sha256()
@@ -558,7 +558,7 @@ def csrc_digest():
     h.update(open(os.path.join(ROOT, "include", "spurfies_hip.h"), "rb").read().split(OTHER_SECTION.encode())[0])
     from spurfies_amd import build as _build
 
-    h.update(" ".join(_build.FLAGS).encode())          # the compiler flags are part of the kernels' identity (round 6: -amdgpu-mfma-vgpr-form)
+    h.update(" ".join(_build.FLAGS).encode())          # the compiler flags are part of the kernels' identity (-amdgpu-mfma-vgpr-form and the like)
     return h.hexdigest()
 
 
